@@ -1,0 +1,423 @@
+"""Timed operators of a decode step whose weights are held in 4 bits and whose cache is held in 8.
+
+``listed()`` names the cases, ``draw(rng)`` gives further sizes of the same ranges, ``prepare(case, seed)``
+builds what a program holds before the call, ``run(state)`` is one pass and ``exact(case, seed)`` the same
+result in 64 bits. With ``own`` set, ``run`` calls the library's entry points; else it computes the operators in
+their plain form, elementary torch operations in 32 bits with one rounding at the end. A case's ``op`` is one of
+
+  linear  y = norm?(x) W^T + residual?, W[n, k] = s[n, k / g] (q[n, k] - z[n, k / g]), q in 0..15 (z = 8 or given)
+  swiglu  silu(norm(x) Wg^T) * (norm(x) Wu^T) with W = cat(Wg, Wu) held the same way
+  write   head norms + RoPE of packed QKV rows, keys and values quantised into an e4m3 cache with one
+          power-of-two scale per block of slots, row and KV head (the block's earlier slots are re-scaled
+          when its scale grows)
+  attend  one-token attention over such a cache (e4m3 or int8), each row at its own position
+
+Weights ~ N(0, 0.02), activations, keys and values ~ N(0, 1), gains ~ 1 + N(0, 0.1), as in ``bench.py``.
+"""
+
+import math
+import sys
+from pathlib import Path
+from types import SimpleNamespace
+
+import torch
+
+own = False
+
+EPS = 1e-6
+THETA = 1e6
+#: Largest value of each 8-bit type that a block's scale maps the block's largest value below.
+TOP = {"e4m3": 448.0, "int8": 127.0}
+TYPES = {"e4m3": torch.float8_e4m3fn, "int8": torch.int8}
+
+
+def listed():
+    return [
+        # The smallest projection: the fused QKV of a small model for one token.
+        dict(name="w4_linear_small_m1", op="linear", m=1, n=4096, k=1024, group=128, zeros=False, norm=True,
+             residual=False),
+        # One user, large model: the down projection, its sum joining the residual stream.
+        dict(name="w4_linear_down_m1", op="linear", m=1, n=4096, k=12288, group=128, zeros=False, norm=False,
+             residual=True),
+        # A batch of sixteen users: QKV of the large model from a checkpoint with zero points and short groups.
+        dict(name="w4_linear_qkv_m16", op="linear", m=16, n=6144, k=4096, group=64, zeros=True, norm=True,
+             residual=False),
+        # An odd size (one GPU's share of an odd vocabulary): nothing is a whole tile.
+        dict(name="w4_linear_odd_m5", op="linear", m=5, n=9497, k=2570, group=32, zeros=False, norm=False,
+             residual=False),
+        # One user, large model: gate/up + SwiGLU, the step's largest matrix.
+        dict(name="w4_swiglu_m1", op="swiglu", m=1, n=24576, k=4096, group=128, zeros=False, norm=True,
+             residual=False),
+        # A wide verify block on the large model.
+        dict(name="w4_swiglu_m24", op="swiglu", m=24, n=24576, k=4096, group=128, zeros=True, norm=True,
+             residual=False),
+        # One token of one user.
+        dict(name="q8_write_b1", op="write", batch=1, tokens=1, capacity=8192, filled=0.7, block=64, q_heads=32,
+             kv_heads=8, dim=128),
+        # Thirty-two users, rows at different places of their caches, heads of 64.
+        dict(name="q8_write_b32_d64", op="write", batch=32, tokens=1, capacity=2048, filled=0.2, block=32, q_heads=14,
+             kv_heads=2, dim=64),
+        # A prompt of 4001 tokens fills the cache of one layer.
+        dict(name="q8_write_prompt", op="write", batch=1, tokens=4001, capacity=4096, filled=1.0, block=128,
+             q_heads=32, kv_heads=8, dim=128),
+        # Four users early in a conversation on a small model with heads of 64, seven to a KV head.
+        dict(name="q8_attend_short", op="attend", batch=4, capacity=777, filled=0.5, block=16, q_heads=14, kv_heads=2,
+             dim=64, kind="int8"),
+        # One user with a long context.
+        dict(name="q8_attend_b1_32k", op="attend", batch=1, capacity=32768, filled=1.0, block=64, q_heads=32,
+             kv_heads=8, dim=128, kind="e4m3"),
+        # A batch whose rows stand at different places of long caches.
+        dict(name="q8_attend_b32_ragged", op="attend", batch=32, capacity=16384, filled=0.1, block=128, q_heads=32,
+             kv_heads=8, dim=128, kind="e4m3"),
+    ]
+
+
+def _log_int(rng, low, high):
+    return int(round(math.exp(rng.uniform(math.log(low), math.log(high)))))
+
+
+def draw(rng):
+    op = rng.choice(["linear", "linear", "swiglu", "write", "attend", "attend"])
+    if op in ("linear", "swiglu"):
+        m = _log_int(rng, 1, 32)
+        k = _log_int(rng, 512, 12288)
+        k = k if rng.random() < 0.2 else 64 * max(1, k // 64)
+        n = _log_int(rng, 512, min(24576, int(24576 * 4096 / k)))
+        n = 2 * max(1, n // 2) if op == "swiglu" else n
+        n = n if rng.random() < 0.3 else 32 * max(1, n // 32)
+        return dict(op=op, m=m, n=n, k=k, group=rng.choice([32, 64, 128, 128]), zeros=rng.random() < 0.3,
+                    norm=op == "swiglu" or rng.random() < 0.4, residual=op == "linear" and rng.random() < 0.4)
+    dim = rng.choice([64, 128, 128])
+    kv_heads = rng.choice([1, 2, 4, 8])
+    heads = dict(q_heads=kv_heads * rng.choice([1, 2, 3, 4, 4, 5, 7, 8]), kv_heads=kv_heads, dim=dim)
+    block = rng.choice([16, 32, 64, 128])
+    if op == "write":
+        prompt = rng.random() < 0.4
+        batch = 1 if prompt else _log_int(rng, 1, 32)
+        tokens = _log_int(rng, 2, 4001) if prompt else 1
+        capacity = block * ((max(256, _log_int(rng, tokens, 4096)) + block - 1) // block)
+        return dict(op=op, batch=batch, tokens=tokens, capacity=max(capacity, block * (-(-tokens // block))),
+                    filled=rng.choice([1.0, 0.5, 0.1]), block=block, **heads)
+    batch = _log_int(rng, 1, 32)
+    most = int(1.0e9 / (2 * batch * kv_heads * dim))
+    return dict(op=op, batch=batch, capacity=_log_int(rng, 64, max(128, min(65536, most))),
+                filled=rng.choice([1.0, 0.5, 0.1, 0.02]), block=block, kind=rng.choice(["e4m3", "int8"]), **heads)
+
+
+def work(case):
+    c = case
+    if c["op"] in ("linear", "swiglu"):
+        groups = -(-c["k"] // c["group"])
+        out = c["n"] // 2 if c["op"] == "swiglu" else c["n"]
+        moved = c["n"] * c["k"] / 2 + (2.5 if c["zeros"] else 2) * c["n"] * groups
+        moved += 2 * c["m"] * (c["k"] + out * (2 if c["residual"] else 1)) + (2 * c["k"] if c["norm"] else 0)
+        return dict(bytes=int(moved), flops=2 * c["m"] * c["n"] * c["k"])
+    if c["op"] == "write":
+        rows = c["batch"] * c["tokens"]
+        blocks = c["batch"] * c["kv_heads"] * (-(-c["tokens"] // c["block"]))
+        heads = 2 * (c["q_heads"] + 2 * c["kv_heads"]) + 2 * c["q_heads"] + 2 * c["kv_heads"]
+        return dict(bytes=rows * c["dim"] * (heads + 4) + 8 * blocks,
+                    flops=10 * rows * c["dim"] * (c["q_heads"] + c["kv_heads"]))
+    slots = int(_positions(c).sum()) + c["batch"]
+    per = 2 * c["kv_heads"] * c["dim"] + 8 * c["kv_heads"] / c["block"]
+    return dict(bytes=int(slots * per) + 4 * c["batch"] * c["q_heads"] * c["dim"],
+                flops=4 * slots * c["q_heads"] * c["dim"])
+
+
+def _positions(c):
+    """Each row's newest slot: from `filled` of its cache up to the whole of it, evenly spread."""
+    last = c["capacity"] - 1
+    first = int(last * c["filled"])
+    if c["batch"] == 1:
+        return torch.tensor([first], dtype=torch.int64)
+    return (first + (last - first) * torch.arange(c["batch"], dtype=torch.int64) // (c["batch"] - 1)).clamp(0, last)
+
+
+# ---- what a program holds before the call ------------------------------------------------------------
+
+
+def _randn(shape, gen, scale=1.0, shift=0.0):
+    return (torch.randn(shape, generator=gen, device="cuda") * scale + shift).to(torch.bfloat16)
+
+
+def _power(amax, top):
+    """The smallest power of two s with amax <= top s (at least 2^-126)."""
+    m, e = torch.frexp(amax)
+    tm, te = math.frexp(top)
+    e = e - te + (m > tm).to(e.dtype)
+    e = torch.where(amax > 0, e, torch.full_like(e, -126)).clamp(min=-126)
+    return torch.ldexp(torch.ones_like(amax), e)
+
+
+def _encode(codes, kind):
+    return codes.round().to(torch.int8) if kind == "int8" else codes.to(torch.float8_e4m3fn)
+
+
+def _cache(c, kind, gen):
+    """A cache of N(0, 1) values quantised block by block: codes [B, Hkv, C, D] and scales [B, Hkv, C / block]."""
+    blocks = -(-c["capacity"] // c["block"])
+    codes, scales = [], []
+    for _ in range(c["batch"]):
+        x = torch.randn((c["kv_heads"], blocks, c["block"], c["dim"]), generator=gen, device="cuda")
+        s = _power(x.abs().amax(dim=(2, 3)), TOP[kind])
+        q = _encode(x / s[:, :, None, None], kind)
+        codes.append(q.view(c["kv_heads"], -1, c["dim"]).view(torch.uint8)[:, : c["capacity"]])
+        scales.append(s)
+    return torch.stack(codes).contiguous().view(TYPES[kind]), torch.stack(scales).contiguous()
+
+
+def _inputs(case, seed):
+    c = case
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    s = SimpleNamespace(case=c)
+    if c["op"] in ("linear", "swiglu"):
+        groups = -(-c["k"] // c["group"])
+        out = c["n"] // 2 if c["op"] == "swiglu" else c["n"]
+        s.x = _randn((c["m"], c["k"]), gen)
+        # Two codes to a byte along K: the even element in the low half.
+        s.codes = torch.randint(0, 256, (c["n"], (c["k"] + 1) // 2), generator=gen, device="cuda", dtype=torch.uint8)
+        spread = torch.rand((c["n"], groups), generator=gen, device="cuda") * 0.5 + 0.75
+        s.scales = (spread * (0.02 / 4.6)).to(torch.bfloat16)
+        s.zeros = torch.randint(5, 11, (c["n"], groups), generator=gen, device="cuda", dtype=torch.uint8) \
+            if c["zeros"] else None
+        s.gain = _randn((c["k"],), gen, 0.1, 1.0) if c["norm"] else None
+        s.residual = _randn((c["m"], out), gen) if c["residual"] else None
+        return s
+    if c["op"] == "write":
+        width = (c["q_heads"] + 2 * c["kv_heads"]) * c["dim"]
+        s.packed = _randn((c["batch"], c["tokens"], width), gen)
+        s.q_norm = SimpleNamespace(weight=_randn((c["dim"],), gen, 0.1, 1.0), variance_epsilon=EPS)
+        s.k_norm = SimpleNamespace(weight=_randn((c["dim"],), gen, 0.1, 1.0), variance_epsilon=EPS)
+        angles = torch.arange(c["capacity"], device="cuda", dtype=torch.float64)[:, None] * \
+            THETA ** (-torch.arange(0, c["dim"], 2, device="cuda", dtype=torch.float64) / c["dim"])
+        angles = torch.cat((angles, angles), dim=1)
+        s.cos, s.sin = angles.cos().to(torch.bfloat16), angles.sin().to(torch.bfloat16)
+        s.keys, s.k_scales = _cache(c, "e4m3", gen)
+        s.values, s.v_scales = _cache(c, "e4m3", gen)
+        s.prompt = c["tokens"] > 1
+        if s.prompt:
+            s.position = torch.arange(c["tokens"], device="cuda")
+            s.cos, s.sin = s.cos[: c["tokens"]].contiguous(), s.sin[: c["tokens"]].contiguous()
+            s.phases = None
+        else:
+            s.position = _positions(c).cuda()
+            s.phases = torch.zeros((c["batch"], 1), dtype=torch.int64, device="cuda")
+        return s
+    s.query = _randn((c["batch"], c["q_heads"], 1, c["dim"]), gen)
+    s.keys, s.k_scales = _cache(c, c["kind"], gen)
+    s.values, s.v_scales = _cache(c, c["kind"], gen)
+    s.position = _positions(c).cuda()
+    s.scale = c["dim"] ** -0.5
+    return s
+
+
+def prepare(case, seed):
+    state = _inputs(case, seed)
+    if own and case["op"] in ("linear", "swiglu"):
+        # The weights laid out once, as a program does when it loads a checkpoint.
+        w4 = _kernels("w4")
+        state.weight = w4.pack_w4(_codes(state), state.scales, state.zeros, group=case["group"],
+                                  gate_up=case["op"] == "swiglu")
+    return state
+
+
+def _kernels(name):
+    package = str(Path(__file__).resolve().parents[1] / "fast-transformer_amd")
+    if package not in sys.path:
+        sys.path.insert(0, package)
+    if name == "w4":
+        from kernels import w4
+        return w4
+    from kernels import cache_q8
+    return cache_q8
+
+
+def _codes(s):
+    return torch.stack((s.codes & 15, s.codes >> 4), dim=-1).flatten(1)[:, : s.case["k"]]
+
+
+# ---- one pass --------------------------------------------------------------------------------------
+
+
+def run(state):
+    return _own(state) if own else _plain(state)
+
+
+def _own(s):
+    c = s.case
+    if c["op"] == "swiglu":
+        return _kernels("w4").gate_up_swiglu_w4(s.x, s.weight, s.gain, EPS)
+    if c["op"] == "linear":
+        w4 = _kernels("w4")
+        if s.gain is not None:
+            y = w4.rms_norm_linear_w4(s.x, s.gain, EPS, s.weight, residual=s.residual)
+        elif s.residual is not None:
+            y = w4.linear_residual_w4(s.x, s.weight, s.residual)
+        else:
+            y = w4.linear_w4(s.x, s.weight)
+        return y
+    q8 = _kernels("cache_q8")
+    if c["op"] == "attend":
+        return q8.decode_attention_q8(s.query, s.keys, s.values, s.k_scales, s.v_scales, s.position, s.scale)
+    query = q8.qk_rope_cache_q8(s.packed, s.q_norm, s.k_norm, s.cos, s.sin, s.position, s.keys, s.values, s.k_scales,
+                                s.v_scales, c["q_heads"], prefill=s.prompt, rows=not s.prompt, phases=s.phases)
+    return dict(query=query, keys=s.keys, values=s.values, k_scales=s.k_scales, v_scales=s.v_scales)
+
+
+def _plain(s):
+    c = s.case
+    if c["op"] in ("linear", "swiglu"):
+        x = s.x.float()
+        if s.gain is not None:
+            x = x * torch.rsqrt(x.square().mean(dim=1, keepdim=True) + EPS) * s.gain.float()
+        pad = s.scales.shape[1] * c["group"] - c["k"]
+        q = torch.nn.functional.pad(_codes(s).float(), (0, pad)).view(c["n"], -1, c["group"])
+        zero = 8.0 if s.zeros is None else s.zeros.float()[:, :, None]
+        w = ((q - zero) * s.scales.float()[:, :, None]).view(c["n"], -1)[:, : c["k"]]
+        y = x @ w.t()
+        if c["op"] == "swiglu":
+            gate, up = y.split(c["n"] // 2, dim=1)
+            y = gate / (1 + torch.exp(-gate)) * up
+        if s.residual is not None:
+            y = y + s.residual.float()
+        return y.to(torch.bfloat16)
+    if c["op"] == "attend":
+        groups = c["batch"] * c["kv_heads"]
+        share = c["q_heads"] // c["kv_heads"]
+        k = _values(s.keys, s.k_scales, c["block"]).view(groups, -1, c["dim"])
+        v = _values(s.values, s.v_scales, c["block"]).view(groups, -1, c["dim"])
+        q = s.query.float().view(groups, share, c["dim"]).transpose(1, 2).contiguous()
+        scores = (k @ q) * s.scale  # [B Hkv, C, G]
+        seen = torch.arange(c["capacity"], device="cuda")[None] <= s.position[:, None]
+        seen = seen.repeat_interleave(c["kv_heads"], dim=0)[:, :, None]
+        scores = torch.where(seen, scores, -math.inf)
+        p = torch.exp(scores - scores.amax(dim=1, keepdim=True))
+        p = p / p.sum(dim=1, keepdim=True)
+        out = p.transpose(1, 2).contiguous() @ v
+        return out.view(c["batch"], 1, c["q_heads"], c["dim"]).to(torch.bfloat16)
+    heads = s.packed.float().view(c["batch"], c["tokens"], -1, c["dim"])
+    q, k, v = heads.split((c["q_heads"], c["kv_heads"], c["kv_heads"]), dim=2)
+    if s.prompt:
+        cos, sin = s.cos.float()[None, :, None], s.sin.float()[None, :, None]
+        first = torch.zeros(c["batch"], dtype=torch.int64, device="cuda")
+    else:
+        at = s.position[:, None] + s.phases
+        cos, sin = s.cos[at].float()[:, :, None], s.sin[at].float()[:, :, None]
+        first = s.position
+    q, k = _rotated(q, s.q_norm.weight.float(), cos, sin), _rotated(k, s.k_norm.weight.float(), cos, sin)
+    _append(s.keys, s.k_scales, k, first, c["block"])
+    _append(s.values, s.v_scales, v, first, c["block"])
+    return dict(query=q.transpose(1, 2).to(torch.bfloat16), keys=s.keys, values=s.values, k_scales=s.k_scales,
+                v_scales=s.v_scales)
+
+
+def _values(codes, scales, block):
+    """The values that the codes stand for, in 32 bits."""
+    wide = scales.repeat_interleave(block, dim=2)[:, :, : codes.shape[2], None]
+    return codes.float() * wide
+
+
+def _rotated(x, gain, cos, sin):
+    x = x / torch.sqrt(x.square().mean(dim=-1, keepdim=True) + EPS) * gain
+    a, b = x.chunk(2, dim=-1)
+    return x * cos + torch.cat((-b, a), dim=-1) * sin
+
+
+def _append(codes, scales, new, first, block):
+    """Tokens `new` [B, T, Hkv, D] into slots first[b] + t: T = 1 anywhere, or T slots from slot 0."""
+    batch, heads, capacity, dim = codes.shape
+    tokens = new.shape[1]
+    count = -(-tokens // block)
+    at = first // block  # the first block touched; with several, block 0
+    cells = codes.view(torch.uint8).view(batch, heads, capacity // block, block, dim)
+    row = torch.arange(batch, device="cuda")[:, None, None]
+    head = torch.arange(heads, device="cuda")[None, :, None]
+    which = at[:, None, None] + torch.arange(count, device="cuda")
+    old = cells[row, head, which].view(codes.dtype)  # [B, Hkv, count, block, D]
+    old_scale = scales[row, head, which]
+    slot = which[..., None] * block + torch.arange(block, device="cuda")
+    token = slot - first[:, None, None, None]
+    fresh = ((token >= 0) & (token < tokens)).expand(batch, heads, count, block)[..., None]
+    kept = (token < 0).expand(batch, heads, count, block)[..., None]
+    token = token.clamp(0, tokens - 1).expand(batch, heads, count, block)
+    value = new.transpose(1, 2)[row[..., None], head[..., None], token]
+    top = torch.where(fresh, value.abs(), 0.0).amax(dim=(3, 4))
+    scale = _power(top, TOP["e4m3"])
+    scale = torch.where(kept.any(dim=3)[..., 0], torch.maximum(scale, old_scale), scale)
+    wide = scale[..., None, None]
+    out = torch.where(fresh, value / wide, old.float() * (old_scale / scale)[..., None, None]).to(codes.dtype)
+    cells[row, head, which] = torch.where(fresh | kept, out.view(torch.uint8), old.view(torch.uint8))
+    scales[row, head, which] = scale
+
+
+# ---- the same results in 64 bits ---------------------------------------------------------------------
+
+
+def exact(case, seed):
+    c, s = case, _inputs(case, seed)
+    if c["op"] in ("linear", "swiglu"):
+        x = s.x.double()
+        if s.gain is not None:
+            x = x / (x.pow(2).mean(dim=1) + EPS).sqrt()[:, None] * s.gain.double()[None]
+        rows = max(1, (1 << 27) // c["k"])
+        parts = []
+        which = torch.arange(c["k"], device="cuda") // c["group"]
+        for i in range(0, c["n"], rows):
+            byte = s.codes[i : i + rows].to(torch.int64)
+            q = torch.empty((byte.shape[0], 2 * byte.shape[1]), dtype=torch.float64, device="cuda")
+            q[:, 0::2], q[:, 1::2] = byte % 16, byte // 16
+            z = 8.0 if s.zeros is None else s.zeros[i : i + rows].double()[:, which]
+            w = s.scales[i : i + rows].double()[:, which] * (q[:, : c["k"]] - z)
+            parts.append((w @ x.t().contiguous()).t())
+        y = torch.cat(parts, dim=1)
+        if c["op"] == "swiglu":
+            gate, up = y[:, : c["n"] // 2], y[:, c["n"] // 2 :]
+            y = gate * torch.sigmoid(gate) * up
+        return y if s.residual is None else y + s.residual.double()
+    if c["op"] == "attend":
+        out = torch.zeros((c["batch"], 1, c["q_heads"], c["dim"]), dtype=torch.float64, device="cuda")
+        share = c["q_heads"] // c["kv_heads"]
+        for b in range(c["batch"]):
+            n = int(s.position[b]) + 1
+            which = torch.arange(n, device="cuda") // c["block"]
+            k = s.keys[b, :, :n].double() * s.k_scales[b].double()[:, which, None]
+            v = s.values[b, :, :n].double() * s.v_scales[b].double()[:, which, None]
+            q = s.query[b, :, 0].double().view(c["kv_heads"], share, c["dim"])
+            for h in range(c["kv_heads"]):
+                p = torch.softmax((q[h] @ k[h].t()) * s.scale, dim=1)
+                out[b, 0, h * share : (h + 1) * share] = p @ v[h]
+        return out
+    heads = s.packed.double().view(c["batch"], c["tokens"], -1, c["dim"])
+    rotate = torch.zeros((c["dim"], c["dim"]), dtype=torch.float64, device="cuda")
+    half = c["dim"] // 2
+    index = torch.arange(half, device="cuda")
+    rotate[index + half, index], rotate[index, index + half] = -1.0, 1.0
+    phase = torch.arange(c["tokens"], device="cuda").expand(c["batch"], -1) if s.prompt else s.position[:, None]
+    cos, sin = s.cos.double()[phase][:, :, None], s.sin.double()[phase][:, :, None]
+
+    def rope(x, gain):
+        x = x / (x.pow(2).sum(dim=-1, keepdim=True) / c["dim"] + EPS).sqrt() * gain.double()
+        return x * cos + (x @ rotate) * sin
+
+    q = rope(heads[:, :, : c["q_heads"]], s.q_norm.weight)
+    k = rope(heads[:, :, c["q_heads"] : c["q_heads"] + c["kv_heads"]], s.k_norm.weight)
+    v = heads[:, :, c["q_heads"] + c["kv_heads"] :]
+    filled = []
+    for codes, scales, new in ((s.keys, s.k_scales, k), (s.values, s.v_scales, v)):
+        wide, scales = codes.double(), scales.double()
+        for b in range(c["batch"]):
+            begin = 0 if s.prompt else int(s.position[b])
+            end = begin + c["tokens"]
+            for at in range(begin // c["block"], (end - 1) // c["block"] + 1):
+                low, high = max(begin, at * c["block"]), min(end, (at + 1) * c["block"])
+                part = new[b, low - begin : high - begin].transpose(0, 1)  # [Hkv, slots, D]
+                top = part.abs().amax(dim=(1, 2))
+                scale = torch.exp2(torch.ceil(torch.log2((top / TOP["e4m3"]).clamp(min=2.0**-126))))
+                if low > at * c["block"]:
+                    scale = torch.maximum(scale, scales[b, :, at])
+                    wide[b, :, at * c["block"] : low] *= (scales[b, :, at] / scale)[:, None, None]
+                wide[b, :, low:high] = part / scale[:, None, None]
+                scales[b, :, at] = scale
+        filled.append((wide, scales))
+    (keys, k_scales), (values, v_scales) = filled
+    return dict(query=q.transpose(1, 2), keys=keys, values=values, k_scales=k_scales, v_scales=v_scales)
