@@ -269,6 +269,7 @@ struct DeviceInfo {
   int ok;
 };
 DeviceInfo device_info();
+int hip_status(hipError_t e);  // FTK_OK, or FTK_ERR_HIP with the error kept for ftk_last_hip_error
 
 bool gemv_supported(int M, int rpw, int unroll, int kw, int epi);
 hipError_t launch_gemv(const ProjArgs& a, int epi, const GemvShape& shape, hipStream_t stream);

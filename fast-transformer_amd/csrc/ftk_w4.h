@@ -1,0 +1,31 @@
+// Arguments of the projections whose weights are held in 4 bits with group scales (ftk_w4.hip).
+#pragma once
+
+#include "ftk_internal.h"
+
+namespace ftk {
+
+// W[n, k] = s[n, k / g] (q[n, k] - z[n, k / g]), laid out in tiles of 16 weight rows and chunks of 128
+// columns. A chunk of a tile is 1 KiB: lane (li, g) = (lane % 16, lane / 16) of a wave has row li's columns
+// 32 s + 8 g + e (e = 0..7) in dword s, column e at bit 4 (e / 2) + 16 (e % 2).
+struct W4Args {
+  const uint16_t* x;       // [M, K] BF16, rows x_stride elements apart, any 2-byte alignment
+  int64_t x_stride;
+  const u32x4_t* codes;    // [tiles][chunks][64]
+  const uint16_t* scales;  // [tiles][chunks][16][S], S = groups per chunk (1, 2, 4)
+  const uint8_t* zeros;    // the same layout, or null: 8 everywhere
+  const uint16_t* add;     // [M, outputs] joining the outputs, or null
+  uint16_t* y;             // [M, outputs] BF16
+  int M, N, K;             // N: outputs of the epilogue (columns of y)
+  int tiles, chunks;
+  int half_scales;         // scales are FP16 (else BF16)
+};
+
+constexpr int kW4Chunk = 128;   // columns of a chunk
+constexpr int kW4Tile = 16;     // weight rows of a tile (SwiGLU: 8 gate rows and the 8 up rows beside them)
+constexpr int kW4MaxRows = 32;  // rows of x
+
+hipError_t launch_w4(const W4Args& a, int subs, bool swiglu, hipStream_t stream);
+hipError_t launch_w4_dequantize(const W4Args& a, int subs, bool swiglu, uint16_t* w, hipStream_t stream);
+
+}  // namespace ftk

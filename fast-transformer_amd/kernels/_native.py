@@ -23,6 +23,8 @@ KIND_AUTO, KIND_GEMV, KIND_MFMA, KIND_GENERIC, KIND_STREAM, KIND_MFMA_STREAM, KI
     KIND_FLOW = range(10)
 ATTN_AUTO, ATTN_ROWS, ATTN_QUAD = range(3)
 ROPE_PREFILL, ROPE_ROWS, ROPE_TABLE = 0x1, 0x2, 0x4
+W4_ROWS, W4_GATE_UP = range(2)
+W4_SCALE_BF16, W4_SCALE_FP16 = range(2)
 MAX_ROWS = 32
 FLOW_MAX_K = 5120  # K a FLOW wave's x registers hold
 
@@ -74,6 +76,13 @@ class AttnPlan(ctypes.Structure):
                 ("grid", _int), ("workspace_bytes", _i64)]
 
 
+class W4(ctypes.Structure):
+    """ftk_w4: a 4-bit weight's tensors and sizes."""
+
+    _fields_ = [("codes", _c_void_p), ("scales", _c_void_p), ("zeros", _c_void_p), ("N", _i64), ("K", _i64),
+                ("group", _int), ("scale_type", _int), ("layout", _int)]
+
+
 # name -> (restype, argtypes), exactly the declarations of include/ftk.h
 SIGNATURES = {
     "ftk_version": (ctypes.c_char_p, []),
@@ -123,6 +132,9 @@ SIGNATURES = {
     "ftk_qk_rope_cache_bf16": (_int, [_c_void_p, _int, _i64, _c_void_p, _c_void_p, _float, _float, _c_void_p,
                                       _c_void_p, _i64, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p,
                                       _i64, _i64, _i64, _i64, _i64, _i64, _int, _c_void_p]),
+    "ftk_w4_project_bf16": (_int, [_c_void_p, _i64, _c_void_p, _float, ctypes.POINTER(W4), _c_void_p, _c_void_p, _i64,
+                                   _c_void_p]),
+    "ftk_w4_dequantize_bf16": (_int, [ctypes.POINTER(W4), _c_void_p, _c_void_p]),
     "ftk_plan_project": (_int, [_i64, _i64, _i64, _int, _int, ctypes.POINTER(Config), ctypes.POINTER(Plan)]),
     "ftk_stream_read": (_int, [_c_void_p, _i64, _c_void_p, _int, _int, _c_void_p]),
     "ftk_plan_coverage": (_int, [ctypes.POINTER(Plan), _i64, _int, ctypes.POINTER(ctypes.c_int32), _i64,
@@ -184,6 +196,19 @@ _raw_stream = torch._C._cuda_getCurrentRawStream
 def stream_of(tensor):
     """hipStream_t of torch's current stream on the tensor's device."""
     return _raw_stream(tensor.get_device())
+
+
+_device = torch._C._cuda_getDevice
+
+
+def call_on(tensor, name, *args):
+    """``call`` with ``tensor``'s device current and its current stream as the last argument."""
+    index = tensor.get_device()
+    if index == _device():
+        call(name, *args, _raw_stream(index))
+    else:
+        with torch.cuda.device(index):
+            call(name, *args, _raw_stream(index))
 
 
 def ptr(tensor):

@@ -399,6 +399,43 @@ int ftk_qk_rope_cache_bf16(const void* packed, int splits, int64_t split_stride,
                            int64_t table_rows, const int64_t* position, const int64_t* phases, void* query,
                            void* keys, void* values, int64_t batch, int64_t tokens, int64_t q_heads,
                            int64_t kv_heads, int64_t capacity, int64_t dim, int mode, void* stream);
+/* ---- projections over weights held in 4 bits ------------------------------------------ */
+/* W[n, k] = s[n, k / group] (q[n, k] - z[n, k / group]), q in 0..15, z = 8 or a given 0..15.
+ * The weight rows are laid out once, in tiles of 16 and chunks of 128 columns (rows and columns
+ * past the matrix hold any codes and scales of zero):
+ *   codes  [tiles][chunks][64][4] uint32: lane (li, g) = (lane % 16, lane / 16) holds row li of the
+ *          tile; its dword s has columns 32 s + 8 g + e (e = 0..7) of the chunk, column e at bit
+ *          4 (e / 2) + 16 (e % 2)
+ *   scales [tiles][chunks][16][128 / group] 16-bit, BF16 or FP16
+ *   zeros  the same layout, bytes, or NULL: z = 8 throughout
+ * Layout FTK_W4_ROWS: tile t's row li is weight row 16 t + li. FTK_W4_GATE_UP, for W = cat(W_gate,
+ * W_up) [2I, K]: rows 0..7 of tile t are gate rows 8 t .. 8 t + 7 and rows 8..15 the same up rows.
+ * No counterpart in the reference, whose weights are BF16. */
+#define FTK_W4_ROWS 0
+#define FTK_W4_GATE_UP 1
+#define FTK_W4_SCALE_BF16 0
+#define FTK_W4_SCALE_FP16 1
+typedef struct ftk_w4 {
+  const void* codes;   /* 16-byte aligned */
+  const void* scales;  /* 8-byte aligned */
+  const void* zeros;   /* 4-byte aligned, or NULL */
+  int64_t N;           /* weight rows (2 I for FTK_W4_GATE_UP) */
+  int64_t K;
+  int group;           /* columns that share a scale: 32, 64 or 128 */
+  int scale_type;
+  int layout;
+} ftk_w4;
+/* y = norm?(x) W^T, then + residual (FTK_W4_ROWS) or SwiGLU (FTK_W4_GATE_UP: y is [M, I], one rounding
+ * of silu(g) u). x [M, K] BF16 with rows x_stride elements apart and any 2-byte alignment; y and residual
+ * (NULL for none; y itself is allowed) [M, N] contiguous, 2-byte aligned. M is 1..FTK_MAX_ROWS; any N and K.
+ * gamma [K] (NULL for none): x is RMS-normalised first, with the roundings of ftk_rms_norm_bf16; where the
+ * launch has no such prologue the call returns FTK_ERR_UNSUPPORTED and launches nothing, and the caller
+ * normalises x with ftk_rms_norm_bf16. */
+int ftk_w4_project_bf16(const void* x, int64_t x_stride, const void* gamma, float eps, const ftk_w4* w,
+                        const void* residual, void* y, int64_t M, void* stream);
+/* W itself in BF16, [N, K] row-major (cat(W_gate, W_up) for FTK_W4_GATE_UP): s (q - z) rounded once. */
+int ftk_w4_dequantize_bf16(const ftk_w4* w, void* out, void* stream);
+
 /* ---- measurement --------------------------------------------------------------- */
 /* A pure streaming read of `bytes` (a multiple of 16, src 16-byte aligned) with the
  * projection kernels' load path: `grid` persistent workgroups of 256 lanes with a
