@@ -112,7 +112,9 @@ __device__ __forceinline__ u32x4_t quad_head_rope(u32x4_t x, u32x4_t g, u32x4_t 
 
 constexpr int kTileSlots = 32;  // cache rows in a unit of the tile kernel
 
-// The tile kernel's launch, for any shape (ftk_attn_tile.hip).
+// The merge of the intervals' partials (`zero`: rows that saw no slot give zeros), and the tile kernel's launch, for
+// any shape (ftk_attn_tile.hip).
+hipError_t launch_attn_merge(const AttnArgs& a, const AttnShape& s, bool zero, hipStream_t stream);
 hipError_t launch_attn_tile(const AttnArgs& a, const AttnShape& s, hipStream_t stream);
 
 }  // namespace ftk

@@ -284,7 +284,8 @@ __global__ __launch_bounds__(64 * W) void attn_quad_kernel(AttnArgs a) {
 constexpr int kMergeWaves = 4;
 constexpr int kMergePre = 8;
 
-template <int D>
+// ZERO: a row that saw no slot gives zeros (else 0 / 0).
+template <int D, bool ZERO>
 __global__ __launch_bounds__(64 * kMergeWaves) void attn_merge_kernel(const float* partial, const float* stats,
                                                                       uint16_t* out, int splits, int groups_per_kv) {
   constexpr int E = D / 64;  // dimensions per lane
@@ -360,6 +361,10 @@ __global__ __launch_bounds__(64 * kMergeWaves) void attn_merge_kernel(const floa
     for (int e = 0; e < E; ++e)
       o[e] = (((num_lds[0][lane * E + e] + num_lds[1][lane * E + e]) + num_lds[2][lane * E + e]) +
               num_lds[3][lane * E + e]) / den;
+    if constexpr (ZERO) {
+#pragma unroll
+      for (int e = 0; e < E; ++e) o[e] = den == 0.f ? 0.f : o[e];
+    }
     if constexpr (E == 2) {
       *reinterpret_cast<uint32_t*>(out + (size_t)q * D + lane * 2) = pack_bf16(o[0], o[1]);
     } else {
@@ -422,13 +427,16 @@ hipError_t launch_attention(const AttnArgs& a, const AttnShape& s, hipStream_t s
                  : a.packed != nullptr ? launch_quad<true>(args, s, stream)
                                        : launch_quad<false>(args, s, stream);
   if (e != hipSuccess || s.splits == 1) return e;
+  return launch_attn_merge(a, s, false, stream);
+}
+
+hipError_t launch_attn_merge(const AttnArgs& a, const AttnShape& s, bool zero, hipStream_t stream) {
   const unsigned heads = (unsigned)(s.groups * s.group_size);
-  if (s.dim == 128)
-    hipLaunchKernelGGL(attn_merge_kernel<128>, dim3(heads), dim3(64 * kMergeWaves), 0, stream, a.partial, a.stats, a.out, s.splits,
-                       s.group_size);
-  else
-    hipLaunchKernelGGL(attn_merge_kernel<64>, dim3(heads), dim3(64 * kMergeWaves), 0, stream, a.partial, a.stats, a.out, s.splits,
-                       s.group_size);
+  typedef void (*Kernel)(const float*, const float*, uint16_t*, int, int);
+  const Kernel kernel = s.dim == 128 ? (zero ? attn_merge_kernel<128, true> : attn_merge_kernel<128, false>)
+                                     : (zero ? attn_merge_kernel<64, true> : attn_merge_kernel<64, false>);
+  hipLaunchKernelGGL(kernel, dim3(heads), dim3(64 * kMergeWaves), 0, stream, a.partial, a.stats, a.out, s.splits,
+                     s.group_size);
   return hipGetLastError();
 }
 

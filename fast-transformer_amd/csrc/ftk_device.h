@@ -176,6 +176,13 @@ __device__ __forceinline__ u32x4_t load16(const void* p) {
   return *(global_u32x4_t*)p;
 }
 
+// 16 bytes of a pointer aligned to 2: global loads take any alignment (one instruction all the same).
+typedef u32x4_t u32x4_any_t __attribute__((aligned(2)));
+typedef __attribute__((address_space(1))) const u32x4_any_t global_u32x4_any_t;
+__device__ __forceinline__ u32x4_t load16_any(const void* p) {
+  return *(global_u32x4_any_t*)p;
+}
+
 // DPP lane exchange: lanes whose row is masked off read 0.
 template <int CTRL, int ROW_MASK>
 __device__ __forceinline__ float dpp(float v) {

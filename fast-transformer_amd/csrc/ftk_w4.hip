@@ -14,15 +14,13 @@ namespace ftk {
 
 namespace {
 
-typedef u32x4_t u32x4_any_t __attribute__((aligned(2)));
-
 __device__ __forceinline__ float w4_scale(uint32_t bits, bool half) {
   return half ? (float)__builtin_bit_cast(_Float16, (uint16_t)bits) : bf16_to_f32(bits);
 }
 
 // Columns 32 s + 8 g .. + 7 of chunk c of an x row, zero past the row's end.
 __device__ __forceinline__ u32x4_t x_tail(const uint16_t* row, int k, int K) {
-  if (k + 8 <= K) return *(const u32x4_any_t*)(row + k);
+  if (k + 8 <= K) return load16_any(row + k);
   uint32_t o[4] = {0u, 0u, 0u, 0u};
 #pragma unroll
   for (int e = 0; e < 8; ++e)
@@ -98,7 +96,7 @@ __global__ __launch_bounds__(64 * W) void w4_kernel(W4Args a) {
 #pragma unroll
       for (int b = 0; b < CB; ++b)
 #pragma unroll
-        for (int s = 0; s < 4; ++s) x[b][s] = *(const u32x4_any_t*)(xrow[b] + k0 + 32 * s);
+        for (int s = 0; s < 4; ++s) x[b][s] = load16_any(xrow[b] + k0 + 32 * s);
     } else {
 #pragma unroll
       for (int b = 0; b < CB; ++b)

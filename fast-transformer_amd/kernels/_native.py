@@ -23,6 +23,7 @@ KIND_AUTO, KIND_GEMV, KIND_MFMA, KIND_GENERIC, KIND_STREAM, KIND_MFMA_STREAM, KI
     KIND_FLOW = range(10)
 ATTN_AUTO, ATTN_ROWS, ATTN_QUAD = range(3)
 ROPE_PREFILL, ROPE_ROWS, ROPE_TABLE = 0x1, 0x2, 0x4
+Q8_E4M3, Q8_INT8 = range(2)
 W4_ROWS, W4_GATE_UP = range(2)
 W4_SCALE_BF16, W4_SCALE_FP16 = range(2)
 MAX_ROWS = 32
@@ -135,6 +136,14 @@ SIGNATURES = {
     "ftk_w4_project_bf16": (_int, [_c_void_p, _i64, _c_void_p, _float, ctypes.POINTER(W4), _c_void_p, _c_void_p, _i64,
                                    _c_void_p]),
     "ftk_w4_dequantize_bf16": (_int, [ctypes.POINTER(W4), _c_void_p, _c_void_p]),
+    "ftk_qk_rope_cache_q8": (_int, [_c_void_p, _c_void_p, _c_void_p, _float, _float, _c_void_p, _c_void_p, _i64,
+                                    _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _i64,
+                                    _i64, _i64, _i64, _i64, _i64, _i64, _int, _int, _c_void_p]),
+    "ftk_decode_attention_q8": (_int, [_c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _int,
+                                       _c_void_p, _i64, _i64, _i64, _i64, _i64, _i64, _int, ctypes.c_double, _int,
+                                       _c_void_p, _i64, _c_void_p]),
+    "ftk_decode_attention_q8_splits": (_int, [_i64, _i64, _i64, _i64, _i64, _int]),
+    "ftk_decode_attention_q8_workspace_bytes": (_i64, [_i64, _i64, _i64, _i64, _int]),
     "ftk_plan_project": (_int, [_i64, _i64, _i64, _int, _int, ctypes.POINTER(Config), ctypes.POINTER(Plan)]),
     "ftk_stream_read": (_int, [_c_void_p, _i64, _c_void_p, _int, _int, _c_void_p]),
     "ftk_plan_coverage": (_int, [ctypes.POINTER(Plan), _i64, _int, ctypes.POINTER(ctypes.c_int32), _i64,

@@ -436,6 +436,43 @@ int ftk_w4_project_bf16(const void* x, int64_t x_stride, const void* gamma, floa
 /* W itself in BF16, [N, K] row-major (cat(W_gate, W_up) for FTK_W4_GATE_UP): s (q - z) rounded once. */
 int ftk_w4_dequantize_bf16(const ftk_w4* w, void* out, void* stream);
 
+/* ---- the cache held in 8 bits ----------------------------------------------------------- */
+/* Codes [B, Hkv, C, D], one byte each, and an FP32 scale per block of slots of a row and KV head,
+ * [B, Hkv, ceil(C / block)]: slot t's value is code * scale[t / block]. block is 16, 32, 64 or 128; the codes are
+ * 16-byte aligned. No counterpart in the reference, whose cache is BF16. */
+#define FTK_Q8_E4M3 0 /* OCP 8-bit floats, 4 exponent and 3 fraction bits (largest 448; NaN, no infinity) */
+#define FTK_Q8_INT8 1 /* -127..127 */
+/* ftk_qk_rope_cache_bf16 for such caches, with the same modes, positions, phases and tables: head norm + RoPE
+ * of the query heads into query [B, T, Hq, D] (BF16) and of the key heads into `keys`, the value heads into
+ * `values`. FP32 throughout, one rounding of each result. The tokens fill slots position .. position + T - 1;
+ * those outside the cache, and tokens whose phase lies outside the tables, are skipped.
+ * A block's scale is the smallest power of two, at least 2^-126, that keeps its largest finite magnitude within
+ * the codes' range; infinities saturate, NaN is e4m3's NaN and int8's 0. A block's slots before the first new one
+ * keep their values: they hold the block's scale up, and are re-scaled in place when the new slots raise it. A
+ * write to a block's first slot starts its scale anew, and what the slots after the last new one held is lost.
+ * packed [B, T, (Hq + 2 Hkv) D] BF16, gains, tables: any 2-byte alignment; query 16-byte aligned. D is 64 or 128. */
+int ftk_qk_rope_cache_q8(const void* packed, const void* q_gain, const void* k_gain, float q_eps, float k_eps,
+                         const void* cos, const void* sin, int64_t table_rows, const int64_t* position,
+                         const int64_t* phases, void* query, void* keys, void* values, float* k_scales,
+                         float* v_scales, int64_t batch, int64_t tokens, int64_t q_heads, int64_t kv_heads,
+                         int64_t capacity, int64_t dim, int64_t block, int type, int mode, void* stream);
+/* out [B, Hq, D] = softmax(q k^T * scale) v over slots 0..position of each row, BF16 q and out, as
+ * ftk_decode_attention_bf16; a row whose position is below 0 gives zeros. Slots past the position may hold
+ * anything. Any positive scales. D is 64 or 128, Hq / Hkv at most 16, q and out 16-byte aligned. `splits`: slot
+ * intervals per (row, KV head), 0 for the planner's; with more than one, `workspace` holds the partials (16-byte
+ * aligned, its contents before and after the call do not matter). */
+int ftk_decode_attention_q8(const void* q, const void* keys, const void* values, const float* k_scales,
+                            const float* v_scales, const int64_t* position, int positions, void* out, int64_t batch,
+                            int64_t q_heads, int64_t kv_heads, int64_t capacity, int64_t dim, int64_t block,
+                            int type, double scale, int splits, void* workspace, int64_t workspace_bytes,
+                            void* stream);
+/* The intervals of that call on `compute_units` CUs (0: of the current device), and the workspace bytes for so
+ * many (0 for one). -1: a shape the call does not take, or no device. */
+int ftk_decode_attention_q8_splits(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t capacity, int64_t dim,
+                                   int compute_units);
+int64_t ftk_decode_attention_q8_workspace_bytes(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t dim,
+                                                int splits);
+
 /* ---- measurement --------------------------------------------------------------- */
 /* A pure streaming read of `bytes` (a multiple of 16, src 16-byte aligned) with the
  * projection kernels' load path: `grid` persistent workgroups of 256 lanes with a
