@@ -11,6 +11,8 @@ namespace ftk {
 struct W4Args {
   const uint16_t* x;       // [M, K] BF16, rows x_stride elements apart, any 2-byte alignment
   int64_t x_stride;
+  const uint16_t* gain;    // [K]: x is RMS-normalised first; or null
+  float eps;
   const u32x4_t* codes;    // [tiles][chunks][64]
   const uint16_t* scales;  // [tiles][chunks][16][S], S = groups per chunk (1, 2, 4)
   const uint8_t* zeros;    // the same layout, or null: 8 everywhere
@@ -19,13 +21,30 @@ struct W4Args {
   int M, N, K;             // N: outputs of the epilogue (columns of y)
   int tiles, chunks;
   int half_scales;         // scales are FP16 (else BF16)
+  int swiglu;              // tiles of 8 gate and 8 up rows; y = silu(gate) up
+  int rows;                // rows of x to a workgroup (the launch's row blocks: ceil(M / rows))
+  int row_blocks;
 };
 
 constexpr int kW4Chunk = 128;   // columns of a chunk
 constexpr int kW4Tile = 16;     // weight rows of a tile (SwiGLU: 8 gate rows and the 8 up rows beside them)
 constexpr int kW4MaxRows = 32;  // rows of x
 
-hipError_t launch_w4(const W4Args& a, int subs, bool swiglu, hipStream_t stream);
-hipError_t launch_w4_dequantize(const W4Args& a, int subs, bool swiglu, uint16_t* w, hipStream_t stream);
+// A workgroup's waves (they split a row's chunks), and the chunks of a pass where registers do not hold x for them all
+// (half as many for two blocks of operand rows).
+constexpr int kW4Waves = 8, kW4Pass = 4;
+constexpr int kW4Staged = 6;           // operand rows that go through LDS on their way to the registers
+
+// The launch: `held` chunks per wave in registers (streamed: `held` at a time), `blocks` blocks of 16 operand rows.
+struct W4Shape {
+  int held, blocks, grid;
+  bool streamed, few;
+};
+W4Shape w4_shape(W4Args& a, int subs, int cus);
+hipError_t launch_w4_s1(const W4Args& a, const W4Shape& s, hipStream_t stream);  // by groups per chunk
+hipError_t launch_w4_s2(const W4Args& a, const W4Shape& s, hipStream_t stream);
+hipError_t launch_w4_s4(const W4Args& a, const W4Shape& s, hipStream_t stream);
+hipError_t launch_w4(const W4Args& a, int subs, int cus, hipStream_t stream);
+hipError_t launch_w4_dequantize(const W4Args& a, int subs, uint16_t* w, hipStream_t stream);
 
 }  // namespace ftk

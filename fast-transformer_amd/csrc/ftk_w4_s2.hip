@@ -1,0 +1,10 @@
+// The walk's builds with 2 scales to a chunk of 128 columns (groups of 64).
+#include "ftk_w4_walk.h"
+
+namespace ftk {
+
+hipError_t launch_w4_s2(const W4Args& a, const W4Shape& s, hipStream_t stream) {
+  return w4::launch_shape<2>(a, s, stream);
+}
+
+}  // namespace ftk

@@ -1,0 +1,469 @@
+// The walk over 4-bit weight tiles (ftk_w4.hip has the mathematics and the launch rule).
+#pragma once
+
+#include "ftk_dma.h"
+#include "ftk_w4.h"
+
+namespace ftk {
+
+namespace w4 {
+
+__device__ __forceinline__ float scale_f32(uint32_t bits, bool half) {
+  return half ? (float)__builtin_bit_cast(_Float16, (uint16_t)bits) : bf16_to_f32(bits);
+}
+
+__device__ __forceinline__ bool finite_f32(float v) { return (__float_as_uint(v) & 0x7F800000u) != 0x7F800000u; }
+
+// Elements k .. k + 7 of a row of K >= 8, zero past its end: the last 8 of the row (row_part), moved down.
+__device__ __forceinline__ u32x4_t row_part(const uint16_t* row, int k, int K) {
+  return load16_any(row + (k <= K - 8 ? k : K - 8));
+}
+__device__ __forceinline__ u32x4_t row_moved(u32x4_t v, int k, int K) {
+  const int down = k <= K - 8 ? 0 : k - (K - 8);
+  uint64_t lo = v[0] | (uint64_t)v[1] << 32, hi = v[2] | (uint64_t)v[3] << 32;
+  lo = down & 4 ? hi : lo;
+  hi = down & 4 ? 0 : hi;
+  lo = down & 3 ? lo >> 16 * (down & 3) | hi << (64 - 16 * (down & 3)) : lo;
+  hi >>= 16 * (down & 3);
+  lo = down >= 8 ? 0 : lo;
+  hi = down >= 8 ? 0 : hi;
+  return u32x4_t{(uint32_t)lo, (uint32_t)(lo >> 32), (uint32_t)hi, (uint32_t)(hi >> 32)};
+}
+
+// The operand of one step: 128 + q for the 8 codes of a dword. The constants sit in registers (an instruction takes
+// one literal): (v >> 4 i) & mask | ones is a shift and one v_and_or_b32.
+struct Unpack {
+  uint32_t mask = 0x000F000Fu, ones = 0x43004300u;
+  __device__ __forceinline__ Unpack() { asm volatile("" : "+s"(mask), "+v"(ones)); }
+  __device__ __forceinline__ u32x4_t operator()(uint32_t v) const {
+    u32x4_t o;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o[i] = ((v >> (4 * i)) & mask) | ones;
+    return o;
+  }
+};
+
+__device__ __forceinline__ uint32_t code(const W4Args& a, int tile, int li, int k) {
+  const int c = k / kW4Chunk, r = k % kW4Chunk, s = r / 32, g = (r % 32) / 8, e = r % 8;
+  const uint32_t* d = reinterpret_cast<const uint32_t*>(a.codes + ((size_t)tile * a.chunks + c) * 64 + 16 * g + li);
+  return (d[s] >> (4 * (e / 2) + 16 * (e % 2))) & 15u;
+}
+
+// One output's sum element by element, each product s (q - z) x: what the definition says for an x that holds
+// infinities or values whose 128-fold is one.
+template <int S>
+__device__ __forceinline__ float exact_sum(const W4Args& a, int tile, int li, int m) {
+  float sum = 0.f;
+#pragma unroll 1
+  for (int k = 0; k < a.K; ++k) {
+    const size_t at = (((size_t)tile * a.chunks + k / kW4Chunk) * 16 + li) * S + (k % kW4Chunk) * S / kW4Chunk;
+    const float z = a.zeros != nullptr ? (float)a.zeros[at] : 8.f;
+    const float w = ((float)code(a, tile, li, k) - z) * scale_f32(a.scales[at], a.half_scales);
+    float x = bf16_to_f32(a.x[(size_t)m * a.x_stride + k]);
+    if (a.gain != nullptr) x *= bf16_to_f32(a.gain[k]);
+    sum += w * x;
+  }
+  return sum;
+}
+
+// S scales (16 bits each) or zero points (8 bits each) of one row and chunk. Past the tile's range: zeros.
+template <int S>
+struct Scales {
+  uint32_t v[S == 4 ? 2 : 1];
+  __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t rsrc, uint32_t at) {
+    if constexpr (S == 1) {
+      v[0] = __builtin_amdgcn_raw_buffer_load_b16(rsrc, 2 * at, 0, 2);
+    } else if constexpr (S == 2) {
+      v[0] = __builtin_amdgcn_raw_buffer_load_b32(rsrc, 4 * at, 0, 2);
+    } else {
+      const auto p = __builtin_amdgcn_raw_buffer_load_b64(rsrc, 8 * at, 0, 2);
+      v[0] = p[0];
+      v[1] = p[1];
+    }
+  }
+  __device__ __forceinline__ uint32_t get(int s) const { return (v[s >> 1] >> (16 * (s & 1))) & 0xFFFFu; }
+};
+template <int S>
+struct Zeros {
+  uint32_t v;
+  __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t rsrc, uint32_t at) {
+    if constexpr (S == 1)
+      v = __builtin_amdgcn_raw_buffer_load_b8(rsrc, at, 0, 2);
+    else if constexpr (S == 2)
+      v = __builtin_amdgcn_raw_buffer_load_b16(rsrc, 2 * at, 0, 2);
+    else
+      v = __builtin_amdgcn_raw_buffer_load_b32(rsrc, 4 * at, 0, 2);
+  }
+  __device__ __forceinline__ uint32_t get(int s) const { return (v >> (8 * s)) & 0xFFu; }
+};
+
+// Eight x values and the gains they meet as two BF16 addends: the product has 16 significant bits, so the rounded
+// one and what is left of it hold it exactly. `low` (all ones or zero) picks the second.
+__device__ __forceinline__ u32x4_t gained(u32x4_t x, u32x4_t gain, uint32_t low) {
+  float xf[8], gf[8];
+  widen8(x, xf);
+  widen8(gain, gf);
+  u32x4_t o;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float p0 = xf[2 * i] * gf[2 * i], p1 = xf[2 * i + 1] * gf[2 * i + 1];
+    const uint32_t hi = rne_pair(p0, p1) & low;
+    o[i] = rne_pair(p0 - lo_f32(hi), p1 - hi_f32(hi));
+  }
+  return o;
+}
+
+}  // namespace w4
+
+// A workgroup walks tiles walker, walker + walkers, ... Its 8 waves split a tile's chunks (chunk = wave + 8 j), so
+// every wave needs its own chunks of x only. KC: chunks per wave in registers; CB: blocks of 16 operand rows. x is
+// the A operand and the weights the B operand: a lane's accumulators belong to one weight row, one scale serves them.
+// XS: more chunks than registers hold; a tile takes several passes, and x is read again for each.
+// With a gain the operand rows are the rows' x gain as two BF16 addends (rows, then their low parts), and 1 / rms
+// joins in the epilogue: no product waits for the norm's sum, and x gain loses nothing.
+// Rows reach the operand through the wave's own part of LDS: read in the operand's layout, a load touches 16 rows x 64
+// bytes in 64 separate pieces (16 rows of 6144 x 4096: 21 us, most of it those loads); read along the rows, 256 bytes
+// of four at a time, they cost a quarter. FEW (at most kW4Staged operand rows, CB = 1): a load takes a row's four
+// chunks instead. Either way a piece of 8 elements is multiplied by its gain and summed in one lane, once.
+// The weights of the next PF tiles are in flight; x goes out ahead of the first ones, since loads return in order.
+template <int KC, int CB, int S, bool ZP, bool XS, bool FEW>
+__global__ __launch_bounds__(64 * kW4Waves, (KC * CB <= 2 ? 4 : 2)) void w4_walk_kernel(W4Args a) {
+  using namespace w4;
+  static_assert(!FEW || CB == 1, "few rows fill one block");
+  constexpr int W = kW4Waves;
+  constexpr int PF = !XS && (S == 4 ? KC * CB <= 4 : KC * CB <= 6) ? 2 : 1;
+  constexpr int Q = (KC + 3) / 4;  // FEW: pieces of a row per lane
+  __shared__ float red[2][W][16 * CB][17];
+  __shared__ float ssq[W][16 * CB];
+  __shared__ f32x4_t xsum[W][KC * S][4 * CB];  // per group: sums of the operand rows
+  // FEW: pieces [W][KC 16][R]; else a chunk's [W][16 CB rows][16], piece p of row r at place p ^ (r % 16).
+  extern __shared__ u32x4_t dyn[];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int li = lane & 15, g = lane >> 4;
+  const Unpack unpack;
+  // The row blocks of one walk are 8 workgroups apart: on one XCD, whose L2 then serves their weights twice.
+  const int unit = blockIdx.x >> 3, row_block = unit % a.row_blocks;
+  const int walker = (unit / a.row_blocks) * 8 + (blockIdx.x & 7), walkers = gridDim.x / a.row_blocks;
+  const int m0 = row_block * a.rows, rows = a.M - m0 < a.rows ? a.M - m0 : a.rows;
+  const bool norm = a.gain != nullptr;
+  const int operands = norm ? 2 * rows : rows;
+  const u32x4_t one = {0x3F803F80u, 0x3F803F80u, 0x3F803F80u, 0x3F803F80u};
+
+  const uint32_t chunk_bytes = (uint32_t)a.chunks * 1024u;
+  struct Tile {
+    __amdgpu_buffer_rsrc_t codes, scales, zeros;
+  };
+  auto tile_of = [&](int tile) {  // past the last tile: empty ranges, whose loads read nothing
+    const bool there = tile < a.tiles;
+    const size_t block = (size_t)(there ? tile : 0) * a.chunks;
+    Tile t;
+    t.codes = __builtin_amdgcn_make_buffer_rsrc((void*)(a.codes + block * 64), 0, there ? chunk_bytes : 0u, kBufferFlags);
+    t.scales = __builtin_amdgcn_make_buffer_rsrc((void*)(a.scales + block * 16 * S), 0,
+                                                 there ? (uint32_t)a.chunks * 32u * S : 0u, kBufferFlags);
+    if constexpr (ZP)
+      t.zeros = __builtin_amdgcn_make_buffer_rsrc((void*)(a.zeros + block * 16 * S), 0,
+                                                  there ? (uint32_t)a.chunks * 16u * S : 0u, kBufferFlags);
+    return t;
+  };
+  u32x4_t w[PF][KC];
+  Scales<S> sc[PF][KC];
+  Zeros<S> zp[PF][KC];
+  auto load_weights = [&](const Tile& t, int f, int j, int chunk) {
+    w[f][j] = buffer_load16(t.codes, (uint32_t)chunk * 1024u + 16u * lane);
+    sc[f][j].load(t.scales, (uint32_t)chunk * 16u + li);
+    if constexpr (ZP) zp[f][j].load(t.zeros, (uint32_t)chunk * 16u + li);
+  };
+
+  u32x4_t x[CB][XS && !FEW ? 1 : KC][4];
+
+  // FEW: raw pieces of a pass (chunk wave + 8 (4 q + g) of it, piece li), and their way into the operand.
+  u32x4_t raw[FEW ? kW4Staged : 1][Q], raw_gain[Q];
+  u32x4_t* const pieces = dyn + (FEW ? (size_t)wave * KC * 16 * operands : 0);
+  auto piece_k = [&](int pass, int q) { return (pass * KC * W + wave + W * (4 * q + g)) * kW4Chunk + 8 * li; };
+  auto load_pieces = [&](int pass) {
+    if constexpr (FEW) {
+#pragma unroll
+      for (int q = 0; q < Q; ++q) {
+        const int k = piece_k(pass, q);
+#pragma unroll
+        for (int i = 0; i < kW4Staged; ++i)
+          if (i < rows) raw[i][q] = row_part(a.x + (size_t)(m0 + i) * a.x_stride, k, a.K);
+        if (norm) raw_gain[q] = row_part(a.gain, k, a.K);
+      }
+    }
+  };
+  auto form_pieces = [&](int pass, bool count) {
+    if constexpr (FEW) {
+#pragma unroll
+      for (int q = 0; q < Q; ++q) {
+        const int k = piece_k(pass, q), j = 4 * q + g;
+        const bool mine = KC % 4 == 0 || j < KC;
+        const u32x4_t gn = norm ? row_moved(raw_gain[q], k, a.K) : one;
+#pragma unroll
+        for (int i = 0; i < kW4Staged; ++i) {
+          if (i >= rows) continue;
+          const u32x4_t v = row_moved(raw[i][q], k, a.K);
+          if (norm && count) {
+            const float squares = wave_sum(sum_squares8(v, 0.f));
+            if (lane == 0) ssq[wave][i] = (q == 0 && pass == 0 ? 0.f : ssq[wave][i]) + squares;
+          }
+          for (int part = 0; part < (norm ? 2 : 1); ++part) {
+            const u32x4_t o = norm ? gained(v, gn, part ? 0xFFFFFFFFu : 0u) : v;
+            const int r = i + (part ? rows : 0);
+            float sum = dot8(o, one, 0.f);  // over the 4, 8 or 16 pieces of a group
+            sum += dpp<0xB1, 0xF>(sum);
+            sum += dpp<0x4E, 0xF>(sum);
+            if constexpr (S < 4) sum += dpp<0x141, 0xF>(sum);
+            if constexpr (S < 2) sum += dpp<0x140, 0xF>(sum);
+            if (mine) {
+              pieces[(16 * j + li) * operands + r] = o;
+              if (li % (16 / S) == 0) reinterpret_cast<float*>(&xsum[wave][j * S + li / (16 / S)][0])[r] = sum;
+            }
+          }
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < KC; ++j)
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+          x[0][j][s] = u32x4_t{};
+          if (li < operands) x[0][j][s] = pieces[(16 * j + 4 * s + g) * operands + li];
+        }
+    }
+  };
+
+  // Many rows: piece li of rows 4 i + g of a chunk. With a gain the low parts follow `lower` rows after the rows.
+  constexpr int I = 4 * CB;  // row quads (with a gain half of them, where CB = 2: the other block holds low parts)
+  const int lower = FEW ? rows : 8 * CB;
+  u32x4_t many[FEW ? 1 : KC][FEW ? 1 : I], many_gain[KC];
+  float ss[I] = {};
+  u32x4_t* const chunk_lds = dyn + (FEW ? 0 : (size_t)wave * 16 * 16 * CB);
+  auto load_chunk = [&](int j, int chunk) {
+    if constexpr (!FEW) {
+      const int k = chunk * kW4Chunk + 8 * li;
+#pragma unroll
+      for (int i = 0; i < I; ++i) {
+        if (4 * i >= rows) continue;
+        const int m = 4 * i + g < rows ? 4 * i + g : rows - 1;
+        many[j][i] = row_part(a.x + (size_t)(m0 + m) * a.x_stride, k, a.K);
+      }
+      if (norm) many_gain[j] = row_part(a.gain, k, a.K);
+    }
+  };
+  auto form_chunk = [&](int j, int chunk, bool count) {
+    if constexpr (!FEW) {
+      const int k = chunk * kW4Chunk + 8 * li;
+      u32x4_t gn = many_gain[j];
+      if ((chunk + 1) * kW4Chunk > a.K) {  // wave-uniform: a row's last chunk and beyond, zeros past its end
+#pragma unroll
+        for (int i = 0; i < I; ++i)
+          if (4 * i < rows) many[j][i] = row_moved(many[j][i], k, a.K);
+        if (norm) gn = row_moved(gn, k, a.K);
+      }
+      auto place = [&](u32x4_t o, int r) {
+        chunk_lds[r * 16 + (li ^ (r & 15))] = o;
+        float sum = dot8(o, one, 0.f);  // over the 4, 8 or 16 pieces of a group
+        sum += dpp<0xB1, 0xF>(sum);
+        sum += dpp<0x4E, 0xF>(sum);
+        if constexpr (S < 4) sum += dpp<0x141, 0xF>(sum);
+        if constexpr (S < 2) sum += dpp<0x140, 0xF>(sum);
+        if (li % (16 / S) == 0) reinterpret_cast<float*>(&xsum[wave][j * S + li / (16 / S)][0])[r] = sum;
+      };
+#pragma unroll
+      for (int i = 0; i < I; ++i) {
+        if (4 * i >= rows) continue;
+        const u32x4_t v = many[j][i];
+        if (norm) {
+          // (With a gain there are at most 8 CB rows: the quads past them are never reached.)
+          if (count) ss[i] = sum_squares8(v, ss[i]);
+          place(gained(v, gn, 0u), 4 * i + g);
+          place(gained(v, gn, 0xFFFFFFFFu), lower + 4 * i + g);
+        } else {
+          place(v, 4 * i + g);
+        }
+      }
+#pragma unroll
+      for (int b = 0; b < CB; ++b)
+#pragma unroll
+        for (int s = 0; s < 4; ++s)
+          x[b][XS ? 0 : j][s] = chunk_lds[(16 * b + li) * 16 + ((4 * s + g) ^ li)];
+    }
+  };
+  auto keep_squares = [&]() {
+#pragma unroll
+    for (int i = 0; i < I; ++i) {
+      float sum = ss[i];
+      sum += dpp<0xB1, 0xF>(sum);
+      sum += dpp<0x4E, 0xF>(sum);
+      sum += dpp<0x141, 0xF>(sum);
+      sum += dpp<0x140, 0xF>(sum);
+      if (li == 0) ssq[wave][4 * i + g] = sum;
+    }
+  };
+
+  const int passes = XS ? (a.chunks + KC * W - 1) / (KC * W) : 1;
+  if constexpr (FEW) {
+    load_pieces(0);
+  } else {
+#pragma unroll
+    for (int j = 0; j < KC; ++j) load_chunk(j, wave + W * j);
+  }
+  asm volatile("" ::: "memory");
+  Tile cur = tile_of(walker);  // the tile whose later passes are loaded next (XS)
+#pragma unroll
+  for (int f = 0; f < PF; ++f) {
+    const Tile t = f == 0 ? cur : tile_of(walker + f * walkers);
+#pragma unroll
+    for (int j = 0; j < KC; ++j) load_weights(t, f, j, wave + W * j);
+  }
+  if constexpr (!XS) {
+    if constexpr (FEW) {
+      form_pieces(0, true);
+    } else {
+#pragma unroll
+      for (int j = 0; j < KC; ++j) {
+        form_chunk(j, wave + W * j, true);
+        __builtin_amdgcn_sched_barrier(0);  // one chunk's temporaries at a time
+      }
+      if (norm) keep_squares();
+    }
+  }
+
+  int buf = 0;
+  for (int base = walker; base < a.tiles; base += PF * walkers) {
+#pragma unroll
+    for (int f = 0; f < PF; ++f) {
+      const int tile = base + f * walkers;
+      if (tile >= a.tiles) break;
+      f32x4_t acc[CB] = {};
+      const Tile next = tile_of(tile + PF * walkers);
+      // Many groups' sums stay in LDS: read for every tile (an index the compiler cannot see through), not kept in
+      // registers over the walk.
+      int part_of = 0;
+      if constexpr (KC * S * CB > 4) asm volatile("" : "+s"(part_of));
+      for (int p = 0; p < passes; ++p) {
+        const bool last = p + 1 == passes;
+        const Tile& from = last ? next : cur;
+        const int first = last ? 0 : (p + 1) * KC * W;  // the pass whose loads go out now
+        if constexpr (FEW && XS) {
+          form_pieces(p, tile == walker);
+          load_pieces(last ? 0 : p + 1);
+        }
+#pragma unroll
+        for (int j = 0; j < KC; ++j) {
+          if constexpr (XS && !FEW) {
+            form_chunk(j, p * KC * W + wave + W * j, tile == walker);
+            load_chunk(j, first + wave + W * j);
+          }
+#pragma unroll
+          for (int s = 0; s < S; ++s) {
+            f32x4_t part[CB];
+            const float scale = scale_f32(sc[f][j].get(s), a.half_scales);
+            const float minus = ZP ? -(128.f + (float)zp[f][j].get(s)) : -136.f;
+#pragma unroll
+            for (int b = 0; b < CB; ++b) part[b] = xsum[wave][j * S + s + part_of][4 * b + g] * minus;
+#pragma unroll
+            for (int i = 4 / S * s; i < 4 / S * (s + 1); ++i) {
+              const uint32_t wv = w[f][j][i];
+              const u32x4_t o = unpack(wv);
+#pragma unroll
+              for (int b = 0; b < CB; ++b) part[b] = mfma16x16x32(x[b][XS && !FEW ? 0 : j][i], o, part[b]);
+            }
+#pragma unroll
+            for (int b = 0; b < CB; ++b) acc[b] += part[b] * scale;
+          }
+          load_weights(from, f, j, first + wave + W * j);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      }
+      cur = next;
+      // Element r of acc[b]: operand row 16 b + 4 g + r, weight row li of the tile.
+#pragma unroll
+      for (int b = 0; b < CB; ++b)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) red[buf][wave][16 * b + 4 * g + r][li] = acc[b][r];
+      if (XS && !FEW && norm && tile == walker) keep_squares();
+      lds_barrier();
+      // (The other buffer is written next; its readers all pass this barrier's successor first.)
+      const int cols = a.swiglu ? 8 : 16;  // outputs of a tile
+      for (int i = threadIdx.x; i < rows * cols; i += 64 * W) {
+        const int col = a.swiglu ? i & 7 : i & 15, r = a.swiglu ? i >> 3 : i >> 4, m = m0 + r;
+        const int n = tile * cols + col;
+        if (n >= a.N) continue;
+        float v = 0.f, u = 0.f, inv = 1.f;
+#pragma unroll
+        for (int wv = 0; wv < W; ++wv) v += red[buf][wv][r][col];
+        if (a.swiglu) {
+#pragma unroll
+          for (int wv = 0; wv < W; ++wv) u += red[buf][wv][r][col + 8];
+        }
+        if (norm) {
+          float sum = 0.f;
+#pragma unroll
+          for (int wv = 0; wv < W; ++wv) {
+            sum += ssq[wv][r];
+            v += red[buf][wv][lower + r][col];
+          }
+          if (a.swiglu) {
+#pragma unroll
+            for (int wv = 0; wv < W; ++wv) u += red[buf][wv][lower + r][col + 8];
+          }
+          inv = 1.0f / sqrtf(sum / (float)a.K + a.eps);
+        }
+        if (!finite_f32(v)) v = exact_sum<S>(a, tile, col, m);
+        v *= inv;
+        if (a.swiglu) {
+          if (!finite_f32(u)) u = exact_sum<S>(a, tile, col + 8, m);
+          v = silu_f32(v) * (u * inv);
+        }
+        if (a.add != nullptr) v += bf16_to_f32(a.add[(size_t)m * a.N + n]);
+        a.y[(size_t)m * a.N + n] = (uint16_t)f32_to_bf16(v);
+      }
+      buf ^= 1;
+    }
+  }
+}
+
+namespace w4 {
+
+template <int KC, int CB, int S, bool XS, bool FEW>
+void launch(const W4Args& a, const W4Shape& s, hipStream_t stream) {
+  const int operands = (a.gain != nullptr ? 2 : 1) * a.rows;
+  const size_t lds = kW4Waves * 256 * (FEW ? (size_t)KC * operands : (size_t)16 * CB);
+  if (a.zeros != nullptr)
+    hipLaunchKernelGGL((w4_walk_kernel<KC, CB, S, true, XS, FEW>), dim3(s.grid), dim3(64 * kW4Waves), lds, stream, a);
+  else
+    hipLaunchKernelGGL((w4_walk_kernel<KC, CB, S, false, XS, FEW>), dim3(s.grid), dim3(64 * kW4Waves), lds, stream, a);
+}
+
+// Every launch that w4_shape makes.
+template <int S>
+hipError_t launch_shape(const W4Args& a, const W4Shape& s, hipStream_t stream) {
+  const int key = (s.few ? 2000 : 0) + (s.streamed ? 1000 : 0) + s.blocks * 100 + s.held;
+  switch (key) {
+    case 101: launch<1, 1, S, false, false>(a, s, stream); break;
+    case 102: launch<2, 1, S, false, false>(a, s, stream); break;
+    case 103: launch<3, 1, S, false, false>(a, s, stream); break;
+    case 104: launch<4, 1, S, false, false>(a, s, stream); break;
+    case 106: launch<(S < 4 ? 6 : 4), 1, S, false, false>(a, s, stream); break;
+    case 108: launch<(S < 2 ? 8 : 4), 1, S, false, false>(a, s, stream); break;
+    case 201: launch<1, 2, S, false, false>(a, s, stream); break;
+    case 202: launch<2, 2, S, false, false>(a, s, stream); break;
+    case 204: launch<(S < 4 ? 4 : 2), 2, S, false, false>(a, s, stream); break;
+    case 1104: launch<kW4Pass, 1, S, true, false>(a, s, stream); break;
+    case 1202: launch<kW4Pass / 2, 2, S, true, false>(a, s, stream); break;
+    case 2101: launch<1, 1, S, false, true>(a, s, stream); break;
+    case 2102: launch<2, 1, S, false, true>(a, s, stream); break;
+    case 2103: launch<3, 1, S, false, true>(a, s, stream); break;
+    case 2104: launch<4, 1, S, false, true>(a, s, stream); break;
+    case 2106: launch<(S < 4 ? 6 : 4), 1, S, false, true>(a, s, stream); break;
+    case 2108: launch<(S < 2 ? 8 : 4), 1, S, false, true>(a, s, stream); break;
+    case 3104: launch<kW4Pass, 1, S, true, true>(a, s, stream); break;
+    default: return hipErrorInvalidValue;
+  }
+  return hipGetLastError();
+}
+
+}  // namespace w4
+
+}  // namespace ftk

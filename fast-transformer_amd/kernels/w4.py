@@ -11,7 +11,7 @@ where a weight tensor does in the BF16 functions:
     gate_up_swiglu_w4(x, weight, norm_weight, eps)      silu(xn Wg^T) * (xn Wu^T), W = cat(Wg, Wu)
 
 BF16 activations, FP32 sums, one rounding of the result to BF16 (SwiGLU included: its gate and up sums stay
-FP32). An infinite or NaN activation gives what the products with s (q - z) give. Up to ``linear.MAX_ROWS`` rows
+FP32, and the norm rounds nothing on the way: x gain meets the weights as two BF16 addends that hold it exactly). An infinite or NaN activation gives what the products with s (q - z) give. Up to ``linear.MAX_ROWS`` rows
 run on the 4-bit kernels; more rows (a prompt) take ``dequantize_w4`` and the native GEMM, as ``linear`` sends
 them there. No counterpart in the reference, whose weights are BF16.
 """
@@ -43,7 +43,8 @@ class W4Weight:
         self.rows, self.columns, self.group, self.gate_up = rows, columns, group, gate_up
         self.outputs = rows // 2 if gate_up else rows
         self.device = codes.device
-        self._handle = _native.W4(codes.data_ptr(), scales.data_ptr(), _native.ptr(zeros), rows, columns, group,
+        # (The kernels' rows have at least 8 columns; codes past the weight's own meet zeros.)
+        self._handle = _native.W4(codes.data_ptr(), scales.data_ptr(), _native.ptr(zeros), rows, max(columns, 8), group,
                                   _native.W4_SCALE_FP16 if scales.dtype == torch.float16 else _native.W4_SCALE_BF16,
                                   _native.W4_GATE_UP if gate_up else _native.W4_ROWS)
         self._ref = ctypes.byref(self._handle)
@@ -123,9 +124,9 @@ def quantize_w4(weight, group=128, gate_up=False, scale_dtype=torch.bfloat16):
 def dequantize_w4(weight):
     """The weight itself, BF16 [rows, columns]: each s (q - z) rounded once."""
     _native.require_gpu(weight.codes)
-    out = torch.empty((weight.rows, weight.columns), dtype=torch.bfloat16, device=weight.device)
+    out = torch.empty((weight.rows, weight._handle.K), dtype=torch.bfloat16, device=weight.device)
     _native.call_on(out, "ftk_w4_dequantize_bf16", weight._ref, out.data_ptr())
-    return out
+    return out if weight.columns == weight._handle.K else out[:, : weight.columns].contiguous()
 
 
 def _rows(x, weight):
@@ -159,15 +160,19 @@ def _project(x, weight, norm_weight, eps, residual):
         residual = residual.reshape(rows, weight.outputs).contiguous()
     if norm_weight is not None:
         _like("norm_weight", norm_weight, (weight.columns,), x.device)
-        flat = rms_norm(flat, norm_weight, eps)
+        norm_weight = norm_weight.contiguous()
     if rows > _native.MAX_ROWS:
-        y = F.linear(flat, dequantize_w4(weight))
+        y = F.linear(flat if norm_weight is None else rms_norm(flat, norm_weight, eps), dequantize_w4(weight))
         y = swiglu(y) if weight.gate_up else y if residual is None else y + residual
         return y.view(shape)
     out = torch.empty((rows, weight.outputs), dtype=torch.bfloat16, device=x.device)
     if rows:
-        _native.call_on(out, "ftk_w4_project_bf16", flat.data_ptr(), flat.stride(0), None, float(eps), weight._ref,
-                        None if residual is None else residual.data_ptr(), out.data_ptr(), rows)
+        if norm_weight is not None and weight.columns < 8:
+            flat, norm_weight = rms_norm(flat, norm_weight, eps), None
+        if weight.columns < 8:
+            flat = F.pad(flat, (0, 8 - weight.columns))
+        _native.call_on(out, "ftk_w4_project_bf16", flat.data_ptr(), flat.stride(0), _native.ptr(norm_weight),
+                        float(eps), weight._ref, _native.ptr(residual), out.data_ptr(), rows)
     return out if x.dim() == 2 else out.view(shape)
 
 
@@ -189,7 +194,7 @@ def linear_residual_w4(x, weight, residual):
 
 
 def rms_norm_linear_w4(x, norm_weight, eps, weight, residual=None):
-    """rms_norm(x, norm_weight, eps) @ W.T (+ residual), x normalised with ``kernels.rmsnorm.rms_norm``'s roundings."""
+    """rms_norm(x, norm_weight, eps) @ W.T (+ residual), the norm without intermediate roundings."""
     _plain_rows(weight)
     return _project(x, weight, norm_weight, eps, residual)
 
