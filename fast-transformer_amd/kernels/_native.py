@@ -196,6 +196,22 @@ def try_call(name, *args):
     return status
 
 
+class _Calls:
+    """kernels._calls (csrc/ftk_calls.cpp), loaded at the first call: the few-bits operators without ctypes."""
+
+    def __getattr__(self, name):
+        lib()
+        try:
+            from kernels import _calls
+        except ImportError as error:
+            raise RuntimeError("kernels/_calls.so is missing or does not load: build it with `python "
+                               "fast-transformer_amd/build.py` (or __graft_entry__.build())") from error
+        self.__dict__.update({key: getattr(_calls, key) for key in ("w4", "attend", "write")})
+        return self.__dict__[name]
+
+
+calls = _Calls()
+
 #: The raw handle itself: ``torch.cuda.current_stream`` builds a Stream object for each call, a large
 #: part of an eager launch's host time (with the rest of that path, one small projection launched
 #: eagerly 15.5 -> 10.3 us).

@@ -16,6 +16,7 @@ import torch
 
 from kernels import _native
 
+_calls = _native.calls
 #: Slots that may share a scale, and query heads per KV head the attention takes.
 BLOCKS = (16, 32, 64, 128)
 MAX_GROUP = 16
@@ -77,6 +78,10 @@ def qk_rope_cache_q8(packed, q_norm, k_norm, cos, sin, position, keys, values, k
     """``qk_rope_cache`` into an 8-bit cache: the same arguments and result ([B, Hq, T, D], a view of token-major
     storage), FP32 from the packed BF16 QKV [B, T, (Hq + 2 Hkv) D] to one rounding of each query (BF16), key and value
     (a code). Slots outside the cache, and tokens whose phase lies outside the tables, are skipped."""
+    query = _calls.write(packed, q_norm.weight, k_norm.weight, q_norm.variance_epsilon, k_norm.variance_epsilon, cos, sin,
+                         position, keys, values, k_scales, v_scales, q_heads, prefill, rows, phases)
+    if query is not None:
+        return query
     kind, block = _check(keys, values, k_scales, v_scales)
     batch, kv_heads, capacity, dim = keys.shape
     q_weight, k_weight = q_norm.weight, k_norm.weight
@@ -138,6 +143,9 @@ def decode_attention_q8(query, keys, values, k_scales, v_scales, position, scale
     past the cache sees all of it. Slots after the position may hold anything. FP32 scores and sums; p weights V as
     two BF16 values that carry 16 bits of it. ``splits``: slot intervals per KV head (0: the planner's).
     """
+    out = _calls.attend(query, keys, values, k_scales, v_scales, position, scale, splits)
+    if out is not None:
+        return out
     kind, block = _check(keys, values, k_scales, v_scales)
     batch, kv_heads, capacity, dim = keys.shape
     if query.dtype != torch.bfloat16 or query.dim() != 4 or query.shape[0] != batch or query.shape[2] != 1 or \

@@ -27,6 +27,7 @@ from kernels.swiglu import swiglu
 
 #: Weight rows of a tile and columns of a chunk of the packed layout.
 TILE, CHUNK = 16, 128
+_calls = _native.calls
 #: Group sizes the kernels take; longer groups (multiples of 128, or whole rows) repeat their scale per chunk.
 GROUPS = (32, 64, 128)
 #: Weight elements laid out at a time: bounds the memory ``pack_w4`` needs beside its result.
@@ -48,6 +49,10 @@ class W4Weight:
                                   _native.W4_SCALE_FP16 if scales.dtype == torch.float16 else _native.W4_SCALE_BF16,
                                   _native.W4_GATE_UP if gate_up else _native.W4_ROWS)
         self._ref = ctypes.byref(self._handle)
+        #: What the direct calls take: the handle's address for the products this weight is for (else None), its device.
+        address = ctypes.addressof(self._handle)
+        self._rows, self._gate_up = (None, address) if gate_up else (address, None)
+        self._index = codes.get_device()
 
     def __repr__(self):
         return f"W4Weight({self.rows} x {self.columns}, group {self.group}{', gate_up' if self.gate_up else ''})"
@@ -183,24 +188,36 @@ def _plain_rows(weight):
 
 def linear_w4(x, weight):
     """x [..., K] @ W.T, BF16 [..., N]."""
-    _plain_rows(weight)
-    return _project(x, weight, None, 0.0, None)
+    out = _calls.w4(x, weight._rows, weight._index, weight.outputs, None, 0.0, None)
+    if out is None:
+        _plain_rows(weight)
+        out = _project(x, weight, None, 0.0, None)
+    return out
 
 
 def linear_residual_w4(x, weight, residual):
     """x @ W.T + residual: the add in FP32, before the one rounding."""
-    _plain_rows(weight)
-    return _project(x, weight, None, 0.0, residual)
+    out = _calls.w4(x, weight._rows, weight._index, weight.outputs, None, 0.0, residual)
+    if out is None:
+        _plain_rows(weight)
+        out = _project(x, weight, None, 0.0, residual)
+    return out
 
 
 def rms_norm_linear_w4(x, norm_weight, eps, weight, residual=None):
     """rms_norm(x, norm_weight, eps) @ W.T (+ residual), the norm without intermediate roundings."""
-    _plain_rows(weight)
-    return _project(x, weight, norm_weight, eps, residual)
+    out = _calls.w4(x, weight._rows, weight._index, weight.outputs, norm_weight, eps, residual)
+    if out is None:
+        _plain_rows(weight)
+        out = _project(x, weight, norm_weight, eps, residual)
+    return out
 
 
 def gate_up_swiglu_w4(x, weight, norm_weight=None, eps=1e-6):
     """silu(xn @ Wg.T) * (xn @ Wu.T), xn = x or rms_norm(x), for a weight packed with ``gate_up``; BF16 [..., I]."""
-    if not weight.gate_up:
-        raise ValueError("the weight must be packed with gate_up=True")
-    return _project(x, weight, norm_weight, eps, None)
+    out = _calls.w4(x, weight._gate_up, weight._index, weight.outputs, norm_weight, eps, None)
+    if out is None:
+        if not weight.gate_up:
+            raise ValueError("the weight must be packed with gate_up=True")
+        out = _project(x, weight, norm_weight, eps, None)
+    return out
