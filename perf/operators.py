@@ -15,6 +15,7 @@ their plain form, elementary torch operations in 32 bits with one rounding at th
 Weights ~ N(0, 0.02), activations, keys and values ~ N(0, 1), gains ~ 1 + N(0, 0.1), as in ``bench.py``.
 """
 
+import functools
 import math
 import sys
 from pathlib import Path
@@ -221,7 +222,8 @@ def prepare(case, seed):
     return state
 
 
-def _kernels(name):
+@functools.lru_cache(maxsize=None)
+def _kernels(name):  # imported once, as a program does
     package = str(Path(__file__).resolve().parents[1] / "fast-transformer_amd")
     if package not in sys.path:
         sys.path.insert(0, package)
