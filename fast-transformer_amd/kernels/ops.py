@@ -26,6 +26,11 @@ Registered:
                                                             qk_rope.py:97-129 (one decode step)
   ftk::rope_attend(packed, q_weight, k_weight, q_eps, k_eps, cos, sin, position, keys!, values!, q_heads, scale,
                    phases?)                                 both of the above in one launch (layers.py:51-55, :76)
+  ftk::linear_w4(x, codes, scales, zeros?, rows, columns, group)        kernels/w4.py over a W4Weight's tensors
+  ftk::gate_up_swiglu_w4(x, codes, scales, zeros?, rows, columns, group, norm_weight?, eps)
+  ftk::decode_attention_q8(query, keys, values, k_scales, v_scales, position, scale)   kernels/cache_q8.py
+  ftk::qk_rope_cache_q8(packed, q_weight, k_weight, q_eps, k_eps, cos, sin, position, keys!, values!, k_scales!,
+                        v_scales!, q_heads, phases)                      one decode step
 """
 
 from typing import Optional, Tuple
@@ -34,11 +39,13 @@ import torch
 from torch import Tensor
 
 from kernels import argmax as _argmax
+from kernels import cache_q8 as _q8
 from kernels import decode_attention as _attention
 from kernels import linear as _linear
 from kernels import qk_rope as _rope
 from kernels import rmsnorm as _rmsnorm
 from kernels import swiglu as _swiglu
+from kernels import w4 as _w4
 
 
 class _Norm:
@@ -185,3 +192,56 @@ def rope_attend(packed: Tensor, q_weight: Tensor, k_weight: Tensor, q_eps: float
 @rope_attend.register_fake
 def _(packed, q_weight, k_weight, q_eps, k_eps, cos, sin, position, keys, values, q_heads, scale, phases=None):
     return packed.new_empty((packed.shape[0], 1, q_heads, keys.shape[-1]), dtype=keys.dtype)
+
+
+def _w4_weight(codes, scales, zeros, rows, columns, group, gate_up):
+    return _w4.W4Weight(codes, scales, zeros, rows, columns, group, gate_up)
+
+
+@torch.library.custom_op("ftk::linear_w4", mutates_args=())
+def linear_w4(x: Tensor, codes: Tensor, scales: Tensor, zeros: Optional[Tensor], rows: int, columns: int,
+              group: int) -> Tensor:
+    return _w4.linear_w4(x, _w4_weight(codes, scales, zeros, rows, columns, group, False))
+
+
+@linear_w4.register_fake
+def _(x, codes, scales, zeros, rows, columns, group):
+    return x.new_empty((*x.shape[:-1], rows))
+
+
+@torch.library.custom_op("ftk::gate_up_swiglu_w4", mutates_args=())
+def gate_up_swiglu_w4(x: Tensor, codes: Tensor, scales: Tensor, zeros: Optional[Tensor], rows: int, columns: int,
+                      group: int, norm_weight: Optional[Tensor], eps: float) -> Tensor:
+    return _w4.gate_up_swiglu_w4(x, _w4_weight(codes, scales, zeros, rows, columns, group, True), norm_weight, eps)
+
+
+@gate_up_swiglu_w4.register_fake
+def _(x, codes, scales, zeros, rows, columns, group, norm_weight, eps):
+    return x.new_empty((*x.shape[:-1], rows // 2))
+
+
+@torch.library.custom_op("ftk::decode_attention_q8", mutates_args=())
+def decode_attention_q8(query: Tensor, keys: Tensor, values: Tensor, k_scales: Tensor, v_scales: Tensor,
+                        position: Tensor, scale: float) -> Tensor:
+    return _q8.decode_attention_q8(query, keys, values, k_scales, v_scales, position, scale)
+
+
+@decode_attention_q8.register_fake
+def _(query, keys, values, k_scales, v_scales, position, scale):
+    batch, heads, _, dim = query.shape
+    return query.new_empty((batch, 1, heads, dim))
+
+
+@torch.library.custom_op("ftk::qk_rope_cache_q8", mutates_args=("keys", "values", "k_scales", "v_scales"))
+def qk_rope_cache_q8(packed: Tensor, q_weight: Tensor, k_weight: Tensor, q_eps: float, k_eps: float, cos: Tensor,
+                     sin: Tensor, position: Tensor, keys: Tensor, values: Tensor, k_scales: Tensor, v_scales: Tensor,
+                     q_heads: int, phases: Tensor) -> Tensor:
+    query = _q8.qk_rope_cache_q8(packed, _Norm(q_weight, q_eps), _Norm(k_weight, k_eps), cos, sin, position, keys,
+                                 values, k_scales, v_scales, q_heads, rows=True, phases=phases)
+    return query.transpose(1, 2).contiguous()  # token-major [B, T, Hq, D]: an op returns a fresh tensor
+
+
+@qk_rope_cache_q8.register_fake
+def _(packed, q_weight, k_weight, q_eps, k_eps, cos, sin, position, keys, values, k_scales, v_scales, q_heads, phases):
+    batch, tokens = packed.shape[:2]
+    return packed.new_empty((batch, tokens, q_heads, keys.shape[-1]))

@@ -40,6 +40,19 @@ class W4Weight:
     the product ends in SwiGLU. Made by ``pack_w4``; its tensors must not be replaced."""
 
     def __init__(self, codes, scales, zeros, rows, columns, group, gate_up):
+        half = TILE // 2 if gate_up else TILE
+        blocks = (-(-(rows // 2 if gate_up else rows) // half), -(-columns // CHUNK))  # tiles, chunks
+        if group not in GROUPS or rows < 1 or columns < 1 or (gate_up and rows % 2):
+            raise ValueError(f"no packed weight of {rows} x {columns} in groups of {group}")
+        if codes.dtype != torch.int32 or codes.shape != (*blocks, 64, 4) or not codes.is_contiguous():
+            raise ValueError(f"codes must be contiguous int32 {(*blocks, 64, 4)}, got {codes.dtype} {tuple(codes.shape)}")
+        shape = (*blocks, TILE, CHUNK // group)
+        for name, t, types in (("scales", scales, (torch.bfloat16, torch.float16)), ("zeros", zeros, (torch.uint8,))):
+            if t is not None and (t.dtype not in types or t.shape != shape or not t.is_contiguous() or
+                                  t.device != codes.device):
+                raise ValueError(f"{name} must be contiguous {shape} beside the codes, got {t.dtype} {tuple(t.shape)}")
+        if any(t is not None and t.data_ptr() % 16 for t in (codes, scales, zeros)):
+            raise ValueError("packed tensors must be 16-byte aligned")
         self.codes, self.scales, self.zeros = codes, scales, zeros
         self.rows, self.columns, self.group, self.gate_up = rows, columns, group, gate_up
         self.outputs = rows // 2 if gate_up else rows
