@@ -48,15 +48,18 @@ int block_log2(int64_t block) {
   return -1;
 }
 
-// Intervals per (row, KV head): two workgroups a CU, each wave of an interval with a unit of its own.
-constexpr int64_t kQ8GroupsPerCu = 2, kQ8Interval = 256;
+// Intervals per (row, KV head): one workgroup a CU, in intervals of at least 256 slots (a unit for each wave); rows of
+// long caches stand at different places, and take intervals of 2048 so that the CUs end together. us: 1 x 8 KV heads
+// x 32K slots 17.2 in 32 intervals, 19.9 / 18.9 in 16 / 64; 1 x 4K 8.9 in 16, 10.1 / 9.1 in 8 / 32; 16 x 4K 27.2 in 2,
+// 30.1 in 1; 32 x 4K (64 heads) 40.1 in 1, 43.9 in 2; 32 x 16K ragged 103 in 8, 113 / 109 in 1 / 16.
+constexpr int64_t kQ8Interval = 256, kQ8LongInterval = 2048, kQ8LongSlots = 8192, kQ8MostIntervals = 64;
 
-int q8_splits(int64_t groups, int64_t capacity, int cus) {
-  const int64_t most = (capacity + kQ8Interval - 1) / kQ8Interval;
-  int64_t splits = kQ8GroupsPerCu * cus / groups;
-  splits = splits < most ? splits : most;
-  splits = splits < kAttnMaxSplits ? splits : kAttnMaxSplits;
-  return (int)(splits < 1 ? 1 : splits);
+int q8_splits(int64_t batch, int64_t kv_heads, int64_t capacity, int cus) {
+  const int64_t fill = cus / (batch * kv_heads), most = (capacity + kQ8Interval - 1) / kQ8Interval;
+  int64_t splits = fill < most ? fill : most;
+  const int64_t many = batch > 1 && capacity >= kQ8LongSlots ? capacity / kQ8LongInterval : 1;
+  splits = splits > many ? splits : many;
+  return (int)(splits < 1 ? 1 : splits > kQ8MostIntervals ? kQ8MostIntervals : splits);
 }
 
 int64_t q8_partials(int64_t batch, int64_t q_heads, int64_t dim, int64_t splits) {
@@ -164,7 +167,7 @@ int ftk_decode_attention_q8_splits(int64_t batch, int64_t q_heads, int64_t kv_he
     if (!d.ok) return -1;
     compute_units = d.cus;
   }
-  return q8_splits(batch * kv_heads, capacity, compute_units);
+  return q8_splits(batch, kv_heads, capacity, compute_units);
 }
 
 int64_t ftk_decode_attention_q8_workspace_bytes(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t dim,
@@ -192,7 +195,7 @@ int ftk_decode_attention_q8(const void* q, const void* keys, const void* values,
   if (splits == 0) {
     const DeviceInfo d = device_info();
     if (!d.ok) return FTK_ERR_INVALID;
-    splits = q8_splits(batch * kv_heads, capacity, d.cus);
+    splits = q8_splits(batch, kv_heads, capacity, d.cus);
   }
   if (batch * kv_heads * splits > INT32_MAX / 2) return FTK_ERR_INVALID;
   if (splits > 1 && (!workspace || !aligned(workspace, 16) || workspace_bytes < q8_partials(batch, q_heads, dim, splits)))
