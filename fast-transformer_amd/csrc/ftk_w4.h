@@ -33,12 +33,11 @@ constexpr int kW4MaxRows = 32;  // rows of x
 // A workgroup's waves (they split a row's chunks), and the chunks of a pass where registers do not hold x for them all
 // (half as many for two blocks of operand rows).
 constexpr int kW4Waves = 8, kW4Pass = 4;
-constexpr int kW4Staged = 6;           // operand rows that go through LDS on their way to the registers
 
 // The launch: `held` chunks per wave in registers (streamed: `held` at a time), `blocks` blocks of 16 operand rows.
 struct W4Shape {
   int held, blocks, grid;
-  bool streamed, few;
+  bool streamed, one;  // passes; a single row of x
 };
 W4Shape w4_shape(W4Args& a, int subs, int cus);
 hipError_t launch_w4_s1(const W4Args& a, const W4Shape& s, hipStream_t stream);  // by groups per chunk

@@ -61,8 +61,8 @@ W4Shape w4_shape(W4Args& a, int subs, int cus) {
     if (s.held != 0 || !built(need, 2)) break;
   }
   s.streamed = s.held == 0;
-  s.few = per * a.rows <= kW4Staged;
-  if (s.streamed) s.held = s.blocks == 1 ? kW4Pass : kW4Pass / 2;
+  s.one = a.M == 1;
+  if (s.streamed) s.held = s.blocks == 2 ? kW4Pass / 2 : s.one && subs < 4 ? 6 : kW4Pass;
   a.row_blocks = (a.M + a.rows - 1) / a.rows;
   // One workgroup to a CU (two where its waves hold few chunks); all walks as even as they come.
   const int slots = cus * (s.held <= 2 && s.blocks == 1 ? 2 : 1) / a.row_blocks;

@@ -66,51 +66,82 @@ __device__ __forceinline__ float exact_sum(const W4Args& a, int tile, int li, in
   return sum;
 }
 
-// S scales (16 bits each) or zero points (8 bits each) of one row and chunk. Past the tile's range: zeros.
-template <int S>
-struct Scales {
-  uint32_t v[S == 4 ? 2 : 1];
+// S scales (16 bits each) or zero points (8 bits each) of one row and chunk. Past the tile's range: zeros. Kept as
+// narrow as they are loaded: widened at the load, they would be waited for there, and every load before them.
+template <int BITS>
+struct Narrow;
+template <>
+struct Narrow<8> {
+  uint8_t v;
   __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t rsrc, uint32_t at) {
-    if constexpr (S == 1) {
-      v[0] = __builtin_amdgcn_raw_buffer_load_b16(rsrc, 2 * at, 0, 2);
-    } else if constexpr (S == 2) {
-      v[0] = __builtin_amdgcn_raw_buffer_load_b32(rsrc, 4 * at, 0, 2);
-    } else {
-      const auto p = __builtin_amdgcn_raw_buffer_load_b64(rsrc, 8 * at, 0, 2);
-      v[0] = p[0];
-      v[1] = p[1];
-    }
+    v = __builtin_amdgcn_raw_buffer_load_b8(rsrc, at, 0, 2);
   }
-  __device__ __forceinline__ uint32_t get(int s) const { return (v[s >> 1] >> (16 * (s & 1))) & 0xFFFFu; }
+  __device__ __forceinline__ uint32_t word(int) const { return v; }
 };
-template <int S>
-struct Zeros {
+template <>
+struct Narrow<16> {
+  uint16_t v;
+  __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t rsrc, uint32_t at) {
+    v = __builtin_amdgcn_raw_buffer_load_b16(rsrc, 2 * at, 0, 2);
+  }
+  __device__ __forceinline__ uint32_t word(int) const { return v; }
+};
+template <>
+struct Narrow<32> {
   uint32_t v;
   __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t rsrc, uint32_t at) {
-    if constexpr (S == 1)
-      v = __builtin_amdgcn_raw_buffer_load_b8(rsrc, at, 0, 2);
-    else if constexpr (S == 2)
-      v = __builtin_amdgcn_raw_buffer_load_b16(rsrc, 2 * at, 0, 2);
-    else
-      v = __builtin_amdgcn_raw_buffer_load_b32(rsrc, 4 * at, 0, 2);
+    v = __builtin_amdgcn_raw_buffer_load_b32(rsrc, 4 * at, 0, 2);
   }
-  __device__ __forceinline__ uint32_t get(int s) const { return (v >> (8 * s)) & 0xFFu; }
+  __device__ __forceinline__ uint32_t word(int) const { return v; }
+};
+template <>
+struct Narrow<64> {
+  u32x2_t v;
+  __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t rsrc, uint32_t at) {
+    v = __builtin_bit_cast(u32x2_t, __builtin_amdgcn_raw_buffer_load_b64(rsrc, 8 * at, 0, 2));
+  }
+  __device__ __forceinline__ uint32_t word(int i) const { return v[i]; }
+};
+template <int S>
+struct Scales : Narrow<16 * S> {
+  __device__ __forceinline__ float get(int s, bool half) const {
+    const uint32_t w = this->word(s >> 1);
+    const float as_half = (float)__builtin_bit_cast(_Float16, (uint16_t)(w >> (16 * (s & 1))));
+    return half ? as_half : s & 1 ? hi_f32(w) : lo_f32(w);
+  }
+};
+template <int S>
+struct Zeros : Narrow<8 * S> {
+  __device__ __forceinline__ uint32_t get(int s) const { return (this->word(0) >> (8 * s)) & 0xFFu; }
 };
 
-// Eight x values and the gains they meet as two BF16 addends: the product has 16 significant bits, so the rounded
-// one and what is left of it hold it exactly. `low` (all ones or zero) picks the second.
-__device__ __forceinline__ u32x4_t gained(u32x4_t x, u32x4_t gain, uint32_t low) {
-  float xf[8], gf[8];
+// Eight x values times their gains as two BF16 addends: the product has 16 significant bits, so the rounded one and
+// what is left of it hold it exactly.
+struct Gained {
+  u32x4_t hi, low;
+};
+__device__ __forceinline__ Gained gained(u32x4_t x, const float (&gain)[8]) {
+  float xf[8];
   widen8(x, xf);
-  widen8(gain, gf);
-  u32x4_t o;
+  Gained o;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const float p0 = xf[2 * i] * gf[2 * i], p1 = xf[2 * i + 1] * gf[2 * i + 1];
-    const uint32_t hi = rne_pair(p0, p1) & low;
-    o[i] = rne_pair(p0 - lo_f32(hi), p1 - hi_f32(hi));
+    const float p0 = xf[2 * i] * gain[2 * i], p1 = xf[2 * i + 1] * gain[2 * i + 1];
+    const uint32_t hi = rne_pair(p0, p1);
+    o.hi[i] = hi;
+    o.low[i] = rne_pair(p0 - lo_f32(hi), p1 - hi_f32(hi));
   }
   return o;
+}
+
+// Sum of a lane's value over the 4, 8 or 16 lanes that hold a group's pieces (S groups to 16 pieces).
+template <int S>
+__device__ __forceinline__ float group_sum(float v) {
+  v += dpp<0xB1, 0xF>(v);
+  v += dpp<0x4E, 0xF>(v);
+  if constexpr (S < 4) v += dpp<0x141, 0xF>(v);
+  if constexpr (S < 2) v += dpp<0x140, 0xF>(v);
+  return v;
 }
 
 }  // namespace w4
@@ -123,20 +154,20 @@ __device__ __forceinline__ u32x4_t gained(u32x4_t x, u32x4_t gain, uint32_t low)
 // joins in the epilogue: no product waits for the norm's sum, and x gain loses nothing.
 // Rows reach the operand through the wave's own part of LDS: read in the operand's layout, a load touches 16 rows x 64
 // bytes in 64 separate pieces (16 rows of 6144 x 4096: 21 us, most of it those loads); read along the rows, 256 bytes
-// of four at a time, they cost a quarter. FEW (at most kW4Staged operand rows, CB = 1): a load takes a row's four
-// chunks instead. Either way a piece of 8 elements is multiplied by its gain and summed in one lane, once.
+// of four at a time, they cost a quarter. ONE (a single row of x, CB = 1): a load takes the row's four chunks instead.
+// Either way a piece of 8 elements is multiplied by its gain and summed in one lane, once.
 // The weights of the next PF tiles are in flight; x goes out ahead of the first ones, since loads return in order.
-template <int KC, int CB, int S, bool ZP, bool XS, bool FEW>
+template <int KC, int CB, int S, bool ZP, bool XS, bool ONE>
 __global__ __launch_bounds__(64 * kW4Waves, (KC * CB <= 2 ? 4 : 2)) void w4_walk_kernel(W4Args a) {
   using namespace w4;
-  static_assert(!FEW || CB == 1, "few rows fill one block");
+  static_assert(!ONE || CB == 1, "one row fills no block");
   constexpr int W = kW4Waves;
-  constexpr int PF = !XS && (S == 4 ? KC * CB <= 4 : KC * CB <= 6) ? 2 : 1;
-  constexpr int Q = (KC + 3) / 4;  // FEW: pieces of a row per lane
+  constexpr int PF = (S == 4 ? KC * CB <= 4 : KC * CB <= 6) && !XS ? 2 : 1;
+  constexpr int Q = ONE ? (KC + 3) / 4 : 1;  // pieces of the row per lane
   __shared__ float red[2][W][16 * CB][17];
   __shared__ float ssq[W][16 * CB];
   __shared__ f32x4_t xsum[W][KC * S][4 * CB];  // per group: sums of the operand rows
-  // FEW: pieces [W][KC 16][R]; else a chunk's [W][16 CB rows][16], piece p of row r at place p ^ (r % 16).
+  // ONE: pieces [W][KC 16][R]; else a chunk's [W][16 CB rows][16], piece p of row r at place p ^ (r % 16).
   extern __shared__ u32x4_t dyn[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int li = lane & 15, g = lane >> 4;
@@ -174,72 +205,87 @@ __global__ __launch_bounds__(64 * kW4Waves, (KC * CB <= 2 ? 4 : 2)) void w4_walk
     if constexpr (ZP) zp[f][j].load(t.zeros, (uint32_t)chunk * 16u + li);
   };
 
-  u32x4_t x[CB][XS && !FEW ? 1 : KC][4];
+  u32x4_t x[CB][XS && !ONE ? 1 : KC][4];
+  if constexpr (ONE) {
+#pragma unroll
+    for (int j = 0; j < KC; ++j)
+#pragma unroll
+      for (int s = 0; s < 4; ++s) x[0][j][s] = u32x4_t{};
+  }
 
-  // FEW: raw pieces of a pass (chunk wave + 8 (4 q + g) of it, piece li), and their way into the operand.
-  u32x4_t raw[FEW ? kW4Staged : 1][Q], raw_gain[Q];
-  u32x4_t* const pieces = dyn + (FEW ? (size_t)wave * KC * 16 * operands : 0);
-  auto piece_k = [&](int pass, int q) { return (pass * KC * W + wave + W * (4 * q + g)) * kW4Chunk + 8 * li; };
+  // With a gain the low parts follow `lower` operand rows after the rows.
+  const int lower = ONE ? rows : 8 * CB;
+
+  // A group's sum of an operand row, times what the accumulators start at (with zero points that is their matter). The
+  // low parts' share is in their row's; theirs is zero.
+  auto keep_sum = [&](int group, int r, float sum) {
+    float* const at = reinterpret_cast<float*>(&xsum[wave][group][0]);
+    at[r] = ZP ? sum : -136.f * sum;
+    if (norm) at[lower + r] = 0.f;
+  };
+
+  // ONE: raw pieces of a pass (chunk wave + 8 (4 q + g) of it, piece li), and their way into the operand.
+  u32x4_t raw[Q], raw_gain[Q];
+  u32x4_t* const pieces = dyn + (ONE ? (size_t)wave * KC * 16 * operands : 0);
+  float row_squares = 0.f;
+  auto piece_chunk = [&](int pass, int q, int g4) { return pass * KC * W + wave + W * (4 * q + g4); };
   auto load_pieces = [&](int pass) {
-    if constexpr (FEW) {
+    if constexpr (ONE) {
 #pragma unroll
       for (int q = 0; q < Q; ++q) {
-        const int k = piece_k(pass, q);
-#pragma unroll
-        for (int i = 0; i < kW4Staged; ++i)
-          if (i < rows) raw[i][q] = row_part(a.x + (size_t)(m0 + i) * a.x_stride, k, a.K);
-        if (norm) raw_gain[q] = row_part(a.gain, k, a.K);
+        const int k = piece_chunk(pass, q, g) * kW4Chunk + 8 * li;
+        raw[q] = row_part(a.x, k, a.K);
+        raw_gain[q] = row_part(norm ? a.gain : a.x, k, a.K);
       }
     }
   };
   auto form_pieces = [&](int pass, bool count) {
-    if constexpr (FEW) {
+    if constexpr (ONE) {
 #pragma unroll
       for (int q = 0; q < Q; ++q) {
-        const int k = piece_k(pass, q), j = 4 * q + g;
+        const int j = 4 * q + g;
+        u32x4_t v = raw[q], gn = raw_gain[q];
+        if ((piece_chunk(pass, q, 3) + 1) * kW4Chunk > a.K) {  // wave-uniform: the row's end is among these chunks
+          const int k = piece_chunk(pass, q, g) * kW4Chunk + 8 * li;
+          v = row_moved(v, k, a.K);
+          gn = row_moved(gn, k, a.K);
+        }
+        float sum;
+        const int at = (16 * j + li) * operands;
         const bool mine = KC % 4 == 0 || j < KC;
-        const u32x4_t gn = norm ? row_moved(raw_gain[q], k, a.K) : one;
-#pragma unroll
-        for (int i = 0; i < kW4Staged; ++i) {
-          if (i >= rows) continue;
-          const u32x4_t v = row_moved(raw[i][q], k, a.K);
-          if (norm && count) {
-            const float squares = wave_sum(sum_squares8(v, 0.f));
-            if (lane == 0) ssq[wave][i] = (q == 0 && pass == 0 ? 0.f : ssq[wave][i]) + squares;
+        if (norm) {
+          float gf[8];
+          widen8(gn, gf);
+          if (count) row_squares = sum_squares8(v, row_squares);
+          const Gained o = gained(v, gf);
+          if (mine) {
+            pieces[at] = o.hi;
+            pieces[at + 1] = o.low;
           }
-          for (int part = 0; part < (norm ? 2 : 1); ++part) {
-            const u32x4_t o = norm ? gained(v, gn, part ? 0xFFFFFFFFu : 0u) : v;
-            const int r = i + (part ? rows : 0);
-            float sum = dot8(o, one, 0.f);  // over the 4, 8 or 16 pieces of a group
-            sum += dpp<0xB1, 0xF>(sum);
-            sum += dpp<0x4E, 0xF>(sum);
-            if constexpr (S < 4) sum += dpp<0x141, 0xF>(sum);
-            if constexpr (S < 2) sum += dpp<0x140, 0xF>(sum);
-            if (mine) {
-              pieces[(16 * j + li) * operands + r] = o;
-              if (li % (16 / S) == 0) reinterpret_cast<float*>(&xsum[wave][j * S + li / (16 / S)][0])[r] = sum;
-            }
-          }
+          sum = dot8(o.low, one, dot8(o.hi, one, 0.f));
+        } else {
+          if (mine) pieces[at] = v;
+          sum = dot8(v, one, 0.f);
         }
+        sum = group_sum<S>(sum);
+        if (mine && li % (16 / S) == 0) keep_sum(j * S + li / (16 / S), 0, sum);
       }
+      if (li < operands) {  // (the other lanes' operands stay zero)
 #pragma unroll
-      for (int j = 0; j < KC; ++j)
+        for (int j = 0; j < KC; ++j)
 #pragma unroll
-        for (int s = 0; s < 4; ++s) {
-          x[0][j][s] = u32x4_t{};
-          if (li < operands) x[0][j][s] = pieces[(16 * j + 4 * s + g) * operands + li];
-        }
+          for (int s = 0; s < 4; ++s) x[0][j][s] = pieces[(16 * j + 4 * s + g) * operands + li];
+      }
     }
   };
 
-  // Many rows: piece li of rows 4 i + g of a chunk. With a gain the low parts follow `lower` rows after the rows.
+  // Many rows: piece li of rows 4 i + g of a chunk.
   constexpr int I = 4 * CB;  // row quads (with a gain half of them, where CB = 2: the other block holds low parts)
-  const int lower = FEW ? rows : 8 * CB;
-  u32x4_t many[FEW ? 1 : KC][FEW ? 1 : I], many_gain[KC];
+  u32x4_t many[ONE ? 1 : KC][ONE ? 1 : I], many_gain[KC];
   float ss[I] = {};
-  u32x4_t* const chunk_lds = dyn + (FEW ? 0 : (size_t)wave * 16 * 16 * CB);
+  u32x4_t* const chunk_lds = dyn + (ONE ? 0 : (size_t)wave * 16 * 16 * CB);
   auto load_chunk = [&](int j, int chunk) {
-    if constexpr (!FEW) {
+    if constexpr (!ONE) {
       const int k = chunk * kW4Chunk + 8 * li;
 #pragma unroll
       for (int i = 0; i < I; ++i) {
@@ -251,7 +297,7 @@ __global__ __launch_bounds__(64 * kW4Waves, (KC * CB <= 2 ? 4 : 2)) void w4_walk
     }
   };
   auto form_chunk = [&](int j, int chunk, bool count) {
-    if constexpr (!FEW) {
+    if constexpr (!ONE) {
       const int k = chunk * kW4Chunk + 8 * li;
       u32x4_t gn = many_gain[j];
       if ((chunk + 1) * kW4Chunk > a.K) {  // wave-uniform: a row's last chunk and beyond, zeros past its end
@@ -260,27 +306,25 @@ __global__ __launch_bounds__(64 * kW4Waves, (KC * CB <= 2 ? 4 : 2)) void w4_walk
           if (4 * i < rows) many[j][i] = row_moved(many[j][i], k, a.K);
         if (norm) gn = row_moved(gn, k, a.K);
       }
-      auto place = [&](u32x4_t o, int r) {
-        chunk_lds[r * 16 + (li ^ (r & 15))] = o;
-        float sum = dot8(o, one, 0.f);  // over the 4, 8 or 16 pieces of a group
-        sum += dpp<0xB1, 0xF>(sum);
-        sum += dpp<0x4E, 0xF>(sum);
-        if constexpr (S < 4) sum += dpp<0x141, 0xF>(sum);
-        if constexpr (S < 2) sum += dpp<0x140, 0xF>(sum);
-        if (li % (16 / S) == 0) reinterpret_cast<float*>(&xsum[wave][j * S + li / (16 / S)][0])[r] = sum;
-      };
+      float gf[8];
+      widen8(gn, gf);
 #pragma unroll
       for (int i = 0; i < I; ++i) {
         if (4 * i >= rows) continue;
         const u32x4_t v = many[j][i];
-        if (norm) {
-          // (With a gain there are at most 8 CB rows: the quads past them are never reached.)
+        const int r = 4 * i + g;
+        float sum;
+        if (norm) {  // (at most 8 CB rows: the quads past them are never reached)
           if (count) ss[i] = sum_squares8(v, ss[i]);
-          place(gained(v, gn, 0u), 4 * i + g);
-          place(gained(v, gn, 0xFFFFFFFFu), lower + 4 * i + g);
+          const Gained o = gained(v, gf);
+          chunk_lds[r * 16 + (li ^ (r & 15))] = o.hi;
+          chunk_lds[(lower + r) * 16 + (li ^ ((lower + r) & 15))] = o.low;
+          sum = group_sum<S>(dot8(o.low, one, dot8(o.hi, one, 0.f)));
         } else {
-          place(v, 4 * i + g);
+          chunk_lds[r * 16 + (li ^ (r & 15))] = v;
+          sum = group_sum<S>(dot8(v, one, 0.f));
         }
+        if (li % (16 / S) == 0) keep_sum(j * S + li / (16 / S), r, sum);
       }
 #pragma unroll
       for (int b = 0; b < CB; ++b)
@@ -290,35 +334,50 @@ __global__ __launch_bounds__(64 * kW4Waves, (KC * CB <= 2 ? 4 : 2)) void w4_walk
     }
   };
   auto keep_squares = [&]() {
+    if constexpr (ONE) {
+      const float sum = wave_sum(row_squares);
+      if (lane == 0) ssq[wave][0] = sum;
+      return;
+    }
 #pragma unroll
     for (int i = 0; i < I; ++i) {
-      float sum = ss[i];
-      sum += dpp<0xB1, 0xF>(sum);
-      sum += dpp<0x4E, 0xF>(sum);
-      sum += dpp<0x141, 0xF>(sum);
-      sum += dpp<0x140, 0xF>(sum);
+      const float sum = group_sum<1>(ss[i]);
       if (li == 0) ssq[wave][4 * i + g] = sum;
     }
   };
 
   const int passes = XS ? (a.chunks + KC * W - 1) / (KC * W) : 1;
-  if constexpr (FEW) {
+  if constexpr (ONE) {
     load_pieces(0);
   } else {
 #pragma unroll
     for (int j = 0; j < KC; ++j) load_chunk(j, wave + W * j);
   }
   asm volatile("" ::: "memory");
-  Tile cur = tile_of(walker);  // the tile whose later passes are loaded next (XS)
+  // Steps (a tile's passes in turn, then the next tile's) PF ahead of the one computed: their tile and pass.
+  int load_tile = walker, load_pass = 0;
+  Tile from = tile_of(walker);
+  auto next_load = [&]() {
+    if (!XS || ++load_pass == passes) {
+      load_pass = 0;
+      load_tile += walkers;
+      from = tile_of(load_tile);
+    }
+  };
 #pragma unroll
   for (int f = 0; f < PF; ++f) {
-    const Tile t = f == 0 ? cur : tile_of(walker + f * walkers);
 #pragma unroll
-    for (int j = 0; j < KC; ++j) load_weights(t, f, j, wave + W * j);
+    for (int j = 0; j < KC; ++j) {
+      load_weights(from, f, j, load_pass * KC * W + wave + W * j);
+      // (In the loop's order: a wait counts the loads behind the one it waits for, on this way into the loop as well.)
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    next_load();
   }
   if constexpr (!XS) {
-    if constexpr (FEW) {
+    if constexpr (ONE) {
       form_pieces(0, true);
+      if (norm) keep_squares();
     } else {
 #pragma unroll
       for (int j = 0; j < KC; ++j) {
@@ -329,64 +388,78 @@ __global__ __launch_bounds__(64 * kW4Waves, (KC * CB <= 2 ? 4 : 2)) void w4_walk
     }
   }
 
-  int buf = 0;
-  for (int base = walker; base < a.tiles; base += PF * walkers) {
+  __shared__ float inverse[16 * CB];  // 1 / rms of the rows, from the first tile on
+  int buf = 0, tile = walker, p = 0, turn = 0;
+  f32x4_t acc[CB] = {};
+  while (tile < a.tiles) {
 #pragma unroll
     for (int f = 0; f < PF; ++f) {
-      const int tile = base + f * walkers;
-      if (tile >= a.tiles) break;
-      f32x4_t acc[CB] = {};
-      const Tile next = tile_of(tile + PF * walkers);
+      // Past the walk's end a step computes nothing, but its loads (of nothing) go out: with an exit here the waits at
+      // the loop's head would allow for the loads of this step only.
+      const bool active = f == 0 || tile < a.tiles;
       // Many groups' sums stay in LDS: read for every tile (an index the compiler cannot see through), not kept in
       // registers over the walk.
       int part_of = 0;
       if constexpr (KC * S * CB > 4) asm volatile("" : "+s"(part_of));
-      for (int p = 0; p < passes; ++p) {
-        const bool last = p + 1 == passes;
-        const Tile& from = last ? next : cur;
-        const int first = last ? 0 : (p + 1) * KC * W;  // the pass whose loads go out now
-        if constexpr (FEW && XS) {
-          form_pieces(p, tile == walker);
-          load_pieces(last ? 0 : p + 1);
-        }
+      if constexpr (ONE && XS) {
+        if (active) form_pieces(p, tile == walker);
+        load_pieces(p + 1 == passes ? 0 : p + 1);
+      }
 #pragma unroll
-        for (int j = 0; j < KC; ++j) {
-          if constexpr (XS && !FEW) {
-            form_chunk(j, p * KC * W + wave + W * j, tile == walker);
-            load_chunk(j, first + wave + W * j);
-          }
+      for (int j = 0; j < KC; ++j) {
+        if constexpr (XS && !ONE) {
+          form_chunk(j, p * KC * W + wave + W * j, tile == walker);
+          load_chunk(j, (p + 1 == passes ? 0 : p + 1) * KC * W + wave + W * j);
+        }
+        if (active) {
+          float scale[S];
+#pragma unroll
+          for (int s = 0; s < S; ++s) scale[s] = sc[f][j].get(s, a.half_scales);
 #pragma unroll
           for (int s = 0; s < S; ++s) {
             f32x4_t part[CB];
-            const float scale = scale_f32(sc[f][j].get(s), a.half_scales);
-            const float minus = ZP ? -(128.f + (float)zp[f][j].get(s)) : -136.f;
 #pragma unroll
-            for (int b = 0; b < CB; ++b) part[b] = xsum[wave][j * S + s + part_of][4 * b + g] * minus;
+            for (int b = 0; b < CB; ++b) {
+              part[b] = xsum[wave][j * S + s + part_of][4 * b + g];
+              if constexpr (ZP) part[b] *= -(128.f + (float)zp[f][j].get(s));
+            }
 #pragma unroll
             for (int i = 4 / S * s; i < 4 / S * (s + 1); ++i) {
               const uint32_t wv = w[f][j][i];
               const u32x4_t o = unpack(wv);
 #pragma unroll
-              for (int b = 0; b < CB; ++b) part[b] = mfma16x16x32(x[b][XS && !FEW ? 0 : j][i], o, part[b]);
+              for (int b = 0; b < CB; ++b) part[b] = mfma16x16x32(x[b][XS && !ONE ? 0 : j][i], o, part[b]);
             }
 #pragma unroll
-            for (int b = 0; b < CB; ++b) acc[b] += part[b] * scale;
+            for (int b = 0; b < CB; ++b) acc[b] += part[b] * scale[s];
           }
-          load_weights(from, f, j, first + wave + W * j);
-          __builtin_amdgcn_sched_barrier(0);
+          // The scales are formed before the loads that replace their words: a word still to be read would be loaded
+          // into another register, and the copy back at the end of the loop waits for every load in flight.
+#pragma unroll
+          for (int s = 0; s < S; ++s) asm volatile("" ::"v"(scale[s]) : "memory");
         }
+        load_weights(from, f, j, load_pass * KC * W + wave + W * j);
+        __builtin_amdgcn_sched_barrier(0);
       }
-      cur = next;
+      next_load();
+      if constexpr (XS) {
+        if (active && ++p < passes) continue;
+        p = 0;
+      }
+      if (!active) continue;
       // Element r of acc[b]: operand row 16 b + 4 g + r, weight row li of the tile.
 #pragma unroll
-      for (int b = 0; b < CB; ++b)
+      for (int b = 0; b < CB; ++b) {
 #pragma unroll
         for (int r = 0; r < 4; ++r) red[buf][wave][16 * b + 4 * g + r][li] = acc[b][r];
-      if (XS && !FEW && norm && tile == walker) keep_squares();
+        acc[b] = f32x4_t{};
+      }
+      if (XS && norm && tile == walker) keep_squares();
       lds_barrier();
-      // (The other buffer is written next; its readers all pass this barrier's successor first.)
+      // (The other buffer is written next; its readers all pass this barrier's successor first. The waves take turns
+      // with a tile's outputs, so that few rows do not always hold up the same one.)
       const int cols = a.swiglu ? 8 : 16;  // outputs of a tile
-      for (int i = threadIdx.x; i < rows * cols; i += 64 * W) {
+      for (int i = (threadIdx.x + 64 * turn) & (64 * W - 1); i < rows * cols; i += 64 * W) {
         const int col = a.swiglu ? i & 7 : i & 15, r = a.swiglu ? i >> 3 : i >> 4, m = m0 + r;
         const int n = tile * cols + col;
         if (n >= a.N) continue;
@@ -398,48 +471,54 @@ __global__ __launch_bounds__(64 * kW4Waves, (KC * CB <= 2 ? 4 : 2)) void w4_walk
           for (int wv = 0; wv < W; ++wv) u += red[buf][wv][r][col + 8];
         }
         if (norm) {
-          float sum = 0.f;
 #pragma unroll
-          for (int wv = 0; wv < W; ++wv) {
-            sum += ssq[wv][r];
-            v += red[buf][wv][lower + r][col];
-          }
+          for (int wv = 0; wv < W; ++wv) v += red[buf][wv][lower + r][col];
           if (a.swiglu) {
 #pragma unroll
             for (int wv = 0; wv < W; ++wv) u += red[buf][wv][lower + r][col + 8];
           }
-          inv = 1.0f / sqrtf(sum / (float)a.K + a.eps);
+          if (tile == walker) {
+            float sum = 0.f;
+#pragma unroll
+            for (int wv = 0; wv < W; ++wv) sum += ssq[wv][r];
+            inv = 1.0f / sqrtf(sum / (float)a.K + a.eps);
+            if (col == 0) inverse[r] = inv;
+          } else {
+            inv = inverse[r];
+          }
         }
-        if (!finite_f32(v)) v = exact_sum<S>(a, tile, col, m);
+        if (__builtin_expect(!finite_f32(v), 0)) v = exact_sum<S>(a, tile, col, m);
         v *= inv;
         if (a.swiglu) {
-          if (!finite_f32(u)) u = exact_sum<S>(a, tile, col + 8, m);
+          if (__builtin_expect(!finite_f32(u), 0)) u = exact_sum<S>(a, tile, col + 8, m);
           v = silu_f32(v) * (u * inv);
         }
         if (a.add != nullptr) v += bf16_to_f32(a.add[(size_t)m * a.N + n]);
         a.y[(size_t)m * a.N + n] = (uint16_t)f32_to_bf16(v);
       }
       buf ^= 1;
+      turn = (turn + 1) & (W - 1);
+      tile += walkers;
     }
   }
 }
 
 namespace w4 {
 
-template <int KC, int CB, int S, bool XS, bool FEW>
+template <int KC, int CB, int S, bool XS, bool ONE>
 void launch(const W4Args& a, const W4Shape& s, hipStream_t stream) {
   const int operands = (a.gain != nullptr ? 2 : 1) * a.rows;
-  const size_t lds = kW4Waves * 256 * (FEW ? (size_t)KC * operands : (size_t)16 * CB);
+  const size_t lds = kW4Waves * 256 * (ONE ? (size_t)KC * operands : (size_t)16 * CB);
   if (a.zeros != nullptr)
-    hipLaunchKernelGGL((w4_walk_kernel<KC, CB, S, true, XS, FEW>), dim3(s.grid), dim3(64 * kW4Waves), lds, stream, a);
+    hipLaunchKernelGGL((w4_walk_kernel<KC, CB, S, true, XS, ONE>), dim3(s.grid), dim3(64 * kW4Waves), lds, stream, a);
   else
-    hipLaunchKernelGGL((w4_walk_kernel<KC, CB, S, false, XS, FEW>), dim3(s.grid), dim3(64 * kW4Waves), lds, stream, a);
+    hipLaunchKernelGGL((w4_walk_kernel<KC, CB, S, false, XS, ONE>), dim3(s.grid), dim3(64 * kW4Waves), lds, stream, a);
 }
 
 // Every launch that w4_shape makes.
 template <int S>
 hipError_t launch_shape(const W4Args& a, const W4Shape& s, hipStream_t stream) {
-  const int key = (s.few ? 2000 : 0) + (s.streamed ? 1000 : 0) + s.blocks * 100 + s.held;
+  const int key = (s.one ? 2000 : 0) + (s.streamed ? 1000 : 0) + s.blocks * 100 + s.held;
   switch (key) {
     case 101: launch<1, 1, S, false, false>(a, s, stream); break;
     case 102: launch<2, 1, S, false, false>(a, s, stream); break;
@@ -458,7 +537,8 @@ hipError_t launch_shape(const W4Args& a, const W4Shape& s, hipStream_t stream) {
     case 2104: launch<4, 1, S, false, true>(a, s, stream); break;
     case 2106: launch<(S < 4 ? 6 : 4), 1, S, false, true>(a, s, stream); break;
     case 2108: launch<(S < 2 ? 8 : 4), 1, S, false, true>(a, s, stream); break;
-    case 3104: launch<kW4Pass, 1, S, true, true>(a, s, stream); break;
+    case 3106: launch<(S < 4 ? 6 : 4), 1, S, true, true>(a, s, stream); break;
+    case 3104: launch<4, 1, S, true, true>(a, s, stream); break;
     default: return hipErrorInvalidValue;
   }
   return hipGetLastError();
