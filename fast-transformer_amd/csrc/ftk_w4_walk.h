@@ -156,13 +156,15 @@ __device__ __forceinline__ float group_sum(float v) {
 // bytes in 64 separate pieces (16 rows of 6144 x 4096: 21 us, most of it those loads); read along the rows, 256 bytes
 // of four at a time, they cost a quarter. ONE (a single row of x, CB = 1): a load takes the row's four chunks instead.
 // Either way a piece of 8 elements is multiplied by its gain and summed in one lane, once.
+// One row with one scale to a chunk and at most 4 chunks takes 128 registers with PF = 1: two workgroups to a CU hide
+// more than two tiles in flight do (24576 x 4096 + norm 12.6 -> 12.1 us, 6144 x 4096 + norm 6.2 -> 6.0).
 // The weights of the next PF tiles are in flight; x goes out ahead of the first ones, since loads return in order.
 template <int KC, int CB, int S, bool ZP, bool XS, bool ONE>
-__global__ __launch_bounds__(64 * kW4Waves, (KC * CB <= 2 ? 4 : 2)) void w4_walk_kernel(W4Args a) {
+__global__ __launch_bounds__(64 * kW4Waves, (KC * CB <= 2 || (ONE && S == 1 && KC <= 4 && !XS) ? 4 : 2)) void w4_walk_kernel(W4Args a) {
   using namespace w4;
   static_assert(!ONE || CB == 1, "one row fills no block");
   constexpr int W = kW4Waves;
-  constexpr int PF = (S == 4 ? KC * CB <= 4 : KC * CB <= 6) && !XS ? 2 : 1;
+  constexpr int PF = (ONE && S == 1 && !XS && KC > 2 && KC <= 4) ? 1 : (S == 4 ? KC * CB <= 4 : KC * CB <= 6) && !XS ? 2 : 1;
   constexpr int Q = ONE ? (KC + 3) / 4 : 1;  // pieces of the row per lane
   __shared__ float red[2][W][16 * CB][17];
   __shared__ float ssq[W][16 * CB];
