@@ -34,6 +34,12 @@ constexpr int kW4MaxRows = 32;  // rows of x
 // (half as many for two blocks of operand rows).
 constexpr int kW4Waves = 8, kW4Pass = 4;
 
+// Builds of 128 registers, two workgroups to a CU: where x takes few of them, and one row with one scale to a chunk. (Three
+// chunks held for several rows fit too, with one tile in flight instead of two: 9497 x 2570 at 5 rows 7.9 -> 8.3 us.)
+constexpr bool w4_pairs(int held, int blocks, int subs, bool streamed, bool one) {
+  return blocks == 1 && !streamed && (held <= 2 || (held <= 4 && subs == 1 && one));
+}
+
 // The launch: `held` chunks per wave in registers (streamed: `held` at a time), `blocks` blocks of 16 operand rows.
 struct W4Shape {
   int held, blocks, grid;

@@ -160,11 +160,11 @@ __device__ __forceinline__ float group_sum(float v) {
 // more than two tiles in flight do (24576 x 4096 + norm 12.6 -> 12.1 us, 6144 x 4096 + norm 6.2 -> 6.0).
 // The weights of the next PF tiles are in flight; x goes out ahead of the first ones, since loads return in order.
 template <int KC, int CB, int S, bool ZP, bool XS, bool ONE>
-__global__ __launch_bounds__(64 * kW4Waves, (KC * CB <= 2 || (ONE && S == 1 && KC <= 4 && !XS) ? 4 : 2)) void w4_walk_kernel(W4Args a) {
+__global__ __launch_bounds__(64 * kW4Waves, (w4_pairs(KC, CB, S, XS, ONE) ? 4 : 2)) void w4_walk_kernel(W4Args a) {
   using namespace w4;
   static_assert(!ONE || CB == 1, "one row fills no block");
   constexpr int W = kW4Waves;
-  constexpr int PF = (ONE && S == 1 && !XS && KC > 2 && KC <= 4) ? 1 : (S == 4 ? KC * CB <= 4 : KC * CB <= 6) && !XS ? 2 : 1;
+  constexpr int PF = w4_pairs(KC, CB, S, XS, ONE) && KC > 2 ? 1 : (S == 4 ? KC * CB <= 4 : KC * CB <= 6) && !XS ? 2 : 1;
   constexpr int Q = ONE ? (KC + 3) / 4 : 1;  // pieces of the row per lane
   __shared__ float red[2][W][16 * CB][17];
   __shared__ float ssq[W][16 * CB];
@@ -258,7 +258,7 @@ __global__ __launch_bounds__(64 * kW4Waves, (KC * CB <= 2 || (ONE && S == 1 && K
         if (norm) {
           float gf[8];
           widen8(gn, gf);
-          if (count) row_squares = sum_squares8(v, row_squares);
+          if (count && mine) row_squares = sum_squares8(v, row_squares);  // (past KC: the next pass's)
           const Gained o = gained(v, gf);
           if (mine) {
             pieces[at] = o.hi;

@@ -101,11 +101,19 @@ def test_gate_up_swiglu(cuda, m, inter, k, group, zeros, norm):
     assert torch.all((got.double() - want).abs() <= bound + 1e-30)
 
 
-@pytest.mark.parametrize("m,n,k", [(1, 512, 1024), (7, 100, 2570), (16, 272, 4096), (32, 33, 512)])
-def test_rms_norm_linear(cuda, m, n, k):
+#: Rows and columns on every path of a launch: one row or several, x held in registers or read in passes, one block of
+#: operand rows or two, one row block or two.
+LAUNCHES = [(1, 512, 1024), (7, 100, 2570), (16, 272, 4096), (32, 33, 512), (1, 40, 9000), (1, 100, 12288), (1, 33, 25000),
+            (2, 40, 9000), (3, 17, 12288), (5, 40, 6200), (9, 40, 4096), (12, 50, 9000), (17, 30, 4096), (24, 64, 12288),
+            (32, 20, 5000), (4, 40, 4700), (8, 24, 8192)]
+
+
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("m,n,k", LAUNCHES)
+def test_rms_norm_linear(cuda, m, n, k, group):
     from kernels.rmsnorm import rms_norm
 
-    weight, *parts = make(n, k, 64, True, cuda)
+    weight, *parts = make(n, k, group, group == 64, cuda)
     x, r = inputs(m, k, cuda), inputs(m, n, cuda, 4)
     gain = (inputs(1, k, cuda, 3)[0].float() * 0.1 + 1).to(torch.bfloat16)
     xn = rms_norm(x, gain, 1e-6)
