@@ -65,8 +65,8 @@ W4Shape w4_shape(W4Args& a, int subs, int cus) {
   if (s.streamed) s.held = s.blocks == 2 ? kW4Pass / 2 : s.one && subs < 4 ? 6 : kW4Pass;
   a.row_blocks = (a.M + a.rows - 1) / a.rows;
   // One workgroup to a CU (two where its waves hold few chunks); all walks as even as they come.
-  const int slots = cus * (w4_pairs(s.held, s.blocks, subs, s.streamed, s.one) ? 2 : 1) / a.row_blocks;
-  const int rounds = (a.tiles + slots - 1) / slots;
+  const int all = cus * (w4_pairs(s.held, s.blocks, subs, s.streamed, s.one) ? 2 : 1) / a.row_blocks;
+  const int slots = all > 0 ? all : 1, rounds = (a.tiles + slots - 1) / slots;
   const int walkers = (a.tiles + rounds - 1) / rounds;
   s.grid = (walkers + 7) / 8 * 8 * a.row_blocks;
   return s;

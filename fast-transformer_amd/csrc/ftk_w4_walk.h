@@ -50,7 +50,8 @@ __device__ __forceinline__ uint32_t code(const W4Args& a, int tile, int li, int 
 }
 
 // One output's sum element by element, each product s (q - z) x: what the definition says for an x that holds
-// infinities or values whose 128-fold is one.
+// infinities or values whose 128-fold is one. (A short loop, not a fast one: with eight elements to a step its registers
+// cost every other call 2 to 6 %; a row that holds NaN takes 2 to 9 ms.)
 template <int S>
 __device__ __forceinline__ float exact_sum(const W4Args& a, int tile, int li, int m) {
   float sum = 0.f;

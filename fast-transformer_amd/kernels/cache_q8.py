@@ -88,6 +88,8 @@ def qk_rope_cache_q8(packed, q_norm, k_norm, cos, sin, position, keys, values, k
     if packed.dim() != 3 or packed.shape[0] != batch or packed.shape[2] != (q_heads + 2 * kv_heads) * dim:
         raise ValueError(f"packed QKV {tuple(packed.shape)} for {batch} rows, {q_heads} + 2 x {kv_heads} heads of {dim}")
     tokens = packed.shape[1]
+    if q_heads < 1 or kv_heads < 1:
+        raise ValueError(f"{q_heads} query and {kv_heads} KV heads: at least one of each")
     for name, t in (("packed", packed), ("cos", cos), ("sin", sin), ("q_norm", q_weight), ("k_norm", k_weight)):
         if t.dtype != torch.bfloat16:
             raise ValueError(f"{name} must be BF16, got {t.dtype}")

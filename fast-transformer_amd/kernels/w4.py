@@ -170,6 +170,10 @@ def _like(name, t, shape, device):
 
 
 def _project(x, weight, norm_weight, eps, residual):
+    """The general call: refusals, copies, rows beyond the kernels', another device than the current one."""
+    if x.is_cuda and x.get_device() != torch.cuda.current_device():
+        with torch.cuda.device(x.device):
+            return _project(x, weight, norm_weight, eps, residual)
     flat = _rows(x, weight)
     rows = flat.shape[0]
     shape = (*x.shape[:-1], weight.outputs)
