@@ -30,9 +30,8 @@ constexpr int kW4Chunk = 128;   // columns of a chunk
 constexpr int kW4Tile = 16;     // weight rows of a tile (SwiGLU: 8 gate rows and the 8 up rows beside them)
 constexpr int kW4MaxRows = 32;  // rows of x
 
-// A workgroup's waves (they split a row's chunks), and the chunks of a pass where registers do not hold x for them all
-// (half as many for two blocks of operand rows).
-constexpr int kW4Waves = 8, kW4Pass = 4;
+// A workgroup's waves: they split a row's chunks.
+constexpr int kW4Waves = 8;
 
 // Builds of 128 registers, two workgroups to a CU: where x takes few of them, and one row with one scale to a chunk. (Three
 // chunks held for several rows fit too, with one tile in flight instead of two: 9497 x 2570 at 5 rows 7.9 -> 8.3 us.)

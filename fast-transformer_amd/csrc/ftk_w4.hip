@@ -42,33 +42,44 @@ __global__ __launch_bounds__(256) void w4_dequantize_kernel(W4Args a, uint16_t* 
 
 // Rows of x to a workgroup, chunks per wave and the grid.
 W4Shape w4_shape(W4Args& a, int subs, int cus) {
-  // The builds, by blocks of 16 operand rows: what the registers of two waves on a SIMD hold (several groups to a
-  // chunk take more of them). With a gain a row has two operand rows (in two halves of the blocks), and more than 16
-  // rows take two row blocks.
+  // The builds: what the registers of two waves on a SIMD hold (several groups to a chunk take more of them).
   static const int held[] = {1, 2, 3, 4, 6, 8};
-  auto built = [&](int h, int blocks) {
-    return blocks == 1 ? h <= (subs == 1 ? 8 : subs == 2 ? 6 : 4) : h != 3 && h <= (subs == 4 ? 2 : 4);
-  };
+  const int most_held = subs == 1 ? 8 : subs == 2 ? 6 : 4;
   const int need = (a.chunks + kW4Waves - 1) / kW4Waves, per = a.gain != nullptr ? 2 : 1;
-  W4Shape s;
-  for (a.row_blocks = 1;; ++a.row_blocks) {
+  // The launch whose workgroups take `blocks` blocks of operand rows (with a gain a row has two), and the tiles that its
+  // longest walk takes.
+  auto shape = [&](int blocks, int& rounds) {
+    W4Shape s;
+    const int most = 16 * blocks / per;
+    a.row_blocks = (a.M + most - 1) / most;
     a.rows = (a.M + a.row_blocks - 1) / a.row_blocks;
-    s.blocks = (per * a.rows + 15) / 16;
-    if (s.blocks > 2) continue;
-    s.held = 0;
-    for (int h : held)
-      if (s.held == 0 && h >= need && built(h, s.blocks)) s.held = h;
-    if (s.held != 0 || !built(need, 2)) break;
+    a.row_blocks = (a.M + a.rows - 1) / a.rows;
+    s.blocks = blocks;
+    s.one = a.M == 1;
+    s.streamed = need > most_held;
+    s.held = blocks == 2 ? 4 : s.one && subs < 4 ? 6 : 4;
+    if (blocks == 1 && !s.streamed)
+      for (const int* h = held; (s.held = *h) < need; ++h) {}
+    // One workgroup to a CU (two where its waves hold few chunks), as many for each row block, by eights; all walks as
+    // even as they come.
+    const int all = cus * (w4_pairs(s.held, s.blocks, subs, s.streamed, s.one) ? 2 : 1) / a.row_blocks / 8 * 8;
+    const int slots = all > 0 ? all : 8;
+    rounds = (a.tiles + slots - 1) / slots;
+    const int walkers = (a.tiles + rounds - 1) / rounds;
+    s.grid = (walkers + 7) / 8 * 8 * a.row_blocks;
+    return s;
+  };
+  int rounds = 0, rounds2 = 0;
+  const W4Shape s = shape(1, rounds);
+  // More rows than a block holds go to several workgroups, which read the weights again from their XCD's L2. Two blocks
+  // to a workgroup halve the walks, but form twice the operand ahead of them and take most of the registers; that pays
+  // from about four tiles fewer on (norm, 16 rows, K = 4096: 24576 outputs 20.7 us by one block, 19.0 by two; 16384:
+  // 15.0, 15.4; 6144: 9.5, 11.6), and only where two blocks leave a wave its 3 or 4 chunks.
+  if (per * a.M > 16 && subs < 4 && (need == 3 || need == 4)) {
+    const W4Shape s2 = shape(2, rounds2);
+    if (rounds - rounds2 > 4) return s2;
+    return shape(1, rounds);
   }
-  s.streamed = s.held == 0;
-  s.one = a.M == 1;
-  if (s.streamed) s.held = s.blocks == 2 ? kW4Pass / 2 : s.one && subs < 4 ? 6 : kW4Pass;
-  a.row_blocks = (a.M + a.rows - 1) / a.rows;
-  // One workgroup to a CU (two where its waves hold few chunks); all walks as even as they come.
-  const int all = cus * (w4_pairs(s.held, s.blocks, subs, s.streamed, s.one) ? 2 : 1) / a.row_blocks;
-  const int slots = all > 0 ? all : 1, rounds = (a.tiles + slots - 1) / slots;
-  const int walkers = (a.tiles + rounds - 1) / rounds;
-  s.grid = (walkers + 7) / 8 * 8 * a.row_blocks;
   return s;
 }
 

@@ -522,6 +522,12 @@ void launch(const W4Args& a, const W4Shape& s, hipStream_t stream) {
 template <int S>
 hipError_t launch_shape(const W4Args& a, const W4Shape& s, hipStream_t stream) {
   const int key = (s.one ? 2000 : 0) + (s.streamed ? 1000 : 0) + s.blocks * 100 + s.held;
+  if constexpr (S < 4) {
+    if (key == 204) {
+      launch<4, 2, S, false, false>(a, s, stream);
+      return hipGetLastError();
+    }
+  }
   switch (key) {
     case 101: launch<1, 1, S, false, false>(a, s, stream); break;
     case 102: launch<2, 1, S, false, false>(a, s, stream); break;
@@ -529,11 +535,7 @@ hipError_t launch_shape(const W4Args& a, const W4Shape& s, hipStream_t stream) {
     case 104: launch<4, 1, S, false, false>(a, s, stream); break;
     case 106: launch<(S < 4 ? 6 : 4), 1, S, false, false>(a, s, stream); break;
     case 108: launch<(S < 2 ? 8 : 4), 1, S, false, false>(a, s, stream); break;
-    case 201: launch<1, 2, S, false, false>(a, s, stream); break;
-    case 202: launch<2, 2, S, false, false>(a, s, stream); break;
-    case 204: launch<(S < 4 ? 4 : 2), 2, S, false, false>(a, s, stream); break;
-    case 1104: launch<kW4Pass, 1, S, true, false>(a, s, stream); break;
-    case 1202: launch<kW4Pass / 2, 2, S, true, false>(a, s, stream); break;
+    case 1104: launch<4, 1, S, true, false>(a, s, stream); break;
     case 2101: launch<1, 1, S, false, true>(a, s, stream); break;
     case 2102: launch<2, 1, S, false, true>(a, s, stream); break;
     case 2103: launch<3, 1, S, false, true>(a, s, stream); break;

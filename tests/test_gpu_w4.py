@@ -108,6 +108,26 @@ LAUNCHES = [(1, 512, 1024), (7, 100, 2570), (16, 272, 4096), (32, 33, 512), (1, 
             (32, 20, 5000), (4, 40, 4700), (8, 24, 8192)]
 
 
+# Enough tiles that a workgroup takes two blocks of operand rows (3 or 4 chunks to a wave), at odd sizes and, for 17 rows
+# and 24 under a norm, with row blocks of unequal rows.
+@pytest.mark.parametrize("norm", [False, True])
+@pytest.mark.parametrize("m,n,k,group", [(17, 19001, 2200, 128), (24, 25003, 3130, 64), (32, 18800, 4096, 128)])
+def test_two_blocks_of_rows(m, n, k, group, norm, cuda):
+    weight, *parts = make(n, k, group, group == 64, cuda)
+    x, r = inputs(m, k, cuda), inputs(m, n, cuda, 4)
+    gain = (inputs(1, k, cuda, 3)[0].float() * 0.1 + 1).to(torch.bfloat16)
+    value, s = wide(*parts)
+    wx = x.double()
+    if norm:
+        wx = wx / torch.sqrt((wx * wx).mean(-1, keepdim=True) + 1e-6) * gain.double()
+        got = w4.rms_norm_linear_w4(x, gain, 1e-6, weight, residual=r)
+    else:
+        got = w4.linear_residual_w4(x, weight, r)
+    want = wx @ value.t().contiguous() + r.double()
+    # (The norm itself: FP32 sums of squares and a root, some roundings of 2^-24 each, within the slack's 2^-16.)
+    assert torch.all((got.double() - want).abs() <= 2.0**-8 * want.abs() + slack(wx, s) + 2.0**-20 * want.abs())
+
+
 @pytest.mark.parametrize("group", [32, 64, 128])
 @pytest.mark.parametrize("m,n,k", LAUNCHES)
 def test_rms_norm_linear(cuda, m, n, k, group):
