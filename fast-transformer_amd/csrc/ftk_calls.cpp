@@ -4,7 +4,7 @@
 // documents (types, shapes, devices, strides), allocates the output and launches. Whatever is not that case -- a wrong
 // type, a view that needs a copy, another device than the current one, no rows -- gives None, nothing launched, and
 // the Python function does the rest: it names what is wrong, or makes the copy. A small call's host time is most of
-// what it takes: 4096 x 1024 at one row 28 us through ctypes, 9 through here, of which the kernel runs 3.7.
+// what it takes: 4096 x 1024 at one row is issued in 4.8 us, 12 less than through ctypes; the kernel runs 3.7.
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
 

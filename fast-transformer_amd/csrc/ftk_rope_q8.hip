@@ -10,6 +10,9 @@
 // A block's slots before the first new one are the valid ones; writing a block's first slot starts its scale anew.
 // One workgroup owns a (row, KV head, block) of K or of V, all of its new slots in registers: no atomics, the result
 // does not depend on any order.
+//
+// A step's write is one launch's start and drain (3.4 us for one row of 48 heads of 128, 3.6 for 32 rows); a prompt's
+// moves its bytes at a copy's rate: 4001 tokens x 48 heads of 128, 92 MB, 18.5 us or 5.0 TB/s.
 #include "../../include/ftk.h"
 #include "ftk_q8.h"
 #include "ftk_rope.h"

@@ -9,6 +9,14 @@
 // The two terms cancel to at most 5 bits of FP32's 24, far below the BF16 rounding of the output.
 // Where x holds an infinity (or 128 x overflows) they meet as inf - inf: an output that is not finite is
 // summed again, element by element (exact_sum).
+//
+// What bounds it (us per graph node, cold weights; in brackets a pure read of the same bytes in one launch): one row of
+// the large matrices the weight read -- 24576 x 4096 + norm + SwiGLU 12.1 (9.5) or 4.3 TB/s, 4096 x 12288 7.6 (5.5); one
+// row of the small ones the launch and the chain x, operand, first product, outputs -- 4096 x 1024 + norm 3.7 (2.2). From
+// about 8 rows on it is the vector unit: x becomes the operand in every workgroup (some 65 instructions for 8 elements
+// of a normalised row), and a tile's codes are unpacked once per row block (7 for 8 codes): 6144 x 4096 + norm at 16 rows
+// 10.7 (3.5), 24576 x 4096 + norm + SwiGLU at 8 / 16 / 24 rows 14.4 / 19.0 / 26.5 (9.6). An operand formed by a launch of
+// its own took that launch's 4 to 5 us again (16 rows of 6144 x 4096 13.3, 24 rows of 24576 x 4096 29.3).
 #include "ftk_w4_walk.h"
 
 namespace ftk {

@@ -11,9 +11,10 @@ where a weight tensor does in the BF16 functions:
     gate_up_swiglu_w4(x, weight, norm_weight, eps)      silu(xn Wg^T) * (xn Wu^T), W = cat(Wg, Wu)
 
 BF16 activations, FP32 sums, one rounding of the result to BF16 (SwiGLU included: its gate and up sums stay
-FP32, and the norm rounds nothing on the way: x gain meets the weights as two BF16 addends that hold it exactly). An infinite or NaN activation gives what the products with s (q - z) give. Up to ``linear.MAX_ROWS`` rows
-run on the 4-bit kernels; more rows (a prompt) take ``dequantize_w4`` and the native GEMM, as ``linear`` sends
-them there. No counterpart in the reference, whose weights are BF16.
+FP32, and the norm rounds nothing on the way: x gain meets the weights as two BF16 addends that hold it exactly).
+An infinite or NaN activation gives what the products with s (q - z) give. Up to ``linear.MAX_ROWS`` rows run on
+the 4-bit kernels; more rows (a prompt) take ``dequantize_w4`` and the native GEMM, as ``linear`` sends them there.
+No counterpart in the reference, whose weights are BF16.
 """
 
 import ctypes

@@ -428,8 +428,8 @@ typedef struct ftk_w4 {
 /* y = norm?(x) W^T, then + residual (FTK_W4_ROWS) or SwiGLU (FTK_W4_GATE_UP: y is [M, I], one rounding
  * of silu(g) u). x [M, K] BF16 with rows x_stride elements apart and any 2-byte alignment; y and residual
  * (NULL for none; y itself is allowed) [M, N] contiguous, 2-byte aligned. M is 1..FTK_MAX_ROWS; any N.
- * gamma [K] (NULL for none): x is RMS-normalised first, x / sqrt(mean(x^2) + eps) gamma, with no rounding on the way (x gamma enters the products as two BF16 addends
- * that hold it exactly, the row's scale joins the FP32 sum). */
+ * gamma [K] (NULL for none): x is RMS-normalised first, x / sqrt(mean(x^2) + eps) gamma, with no rounding on the way
+ * (x gamma enters the products as two BF16 addends that hold it exactly, the row's scale joins the FP32 sum). */
 int ftk_w4_project_bf16(const void* x, int64_t x_stride, const void* gamma, float eps, const ftk_w4* w,
                         const void* residual, void* y, int64_t M, void* stream);
 /* W itself in BF16, [N, K] row-major (cat(W_gate, W_up) for FTK_W4_GATE_UP): s (q - z) rounded once. */
