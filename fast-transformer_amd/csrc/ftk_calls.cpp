@@ -137,7 +137,8 @@ PyObject* attend(PyObject*, PyObject* const* args, Py_ssize_t n) {
   if (!q || !position || !plain(*q, c.device, at::kBFloat16) || !plain(*position, c.device, at::kLong)) Py_RETURN_NONE;
   if (q->dim() != 4 || q->size(0) != c.batch || q->size(2) != 1 || q->size(3) != c.dim || !aligned16(*q)) Py_RETURN_NONE;
   const int64_t heads = q->size(1), positions = position->numel();
-  if (position->dim() != 1 || (positions != 1 && positions != c.batch) || splits < 0) Py_RETURN_NONE;
+  if (position->dim() != 1 || (positions != 1 && positions != c.batch)) Py_RETURN_NONE;
+  if (splits < 0 || splits > INT32_MAX) Py_RETURN_NONE;
   if (splits == 0) splits = ftk_decode_attention_q8_splits(c.batch, heads, c.heads, c.capacity, c.dim, 0);
   if (splits < 1) Py_RETURN_NONE;
   const int64_t need = ftk_decode_attention_q8_workspace_bytes(c.batch, heads, c.heads, c.dim, (int)splits);

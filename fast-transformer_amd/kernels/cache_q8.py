@@ -128,6 +128,8 @@ def qk_rope_cache_q8(packed, q_norm, k_norm, cos, sin, position, keys, values, k
 @functools.lru_cache(maxsize=None)
 def _launch(device, batch, q_heads, kv_heads, capacity, dim, splits):
     """(intervals, workspace bytes) of a shape on a device."""
+    if not 0 <= splits < 1 << 31:
+        raise ValueError(f"{splits} intervals")
     if splits == 0:
         with torch.cuda.device(device):
             splits = _native.lib().ftk_decode_attention_q8_splits(batch, q_heads, kv_heads, capacity, dim, 0)

@@ -132,6 +132,8 @@ def quantize_w4(weight, group=128, gate_up=False, scale_dtype=torch.bfloat16):
     """``weight`` [N, K] rounded to 4 bits, round-to-nearest: per group s = amax / 7 (rounded to ``scale_dtype``),
     q = clamp(round(w / s) + 8, 0, 15), no zero points."""
     n, k = weight.shape
+    if n < 1 or k < 1 or group < 1:
+        raise ValueError(f"a weight of {n} x {k} in groups of {group}")
     groups = -(-k // group)
     wide = F.pad(weight.float(), (0, groups * group - k)).unflatten(1, (groups, group))
     scales = (wide.abs().amax(dim=2) / 7).to(scale_dtype)

@@ -133,3 +133,9 @@ def test_entry_points_refuse_bad_calls():
     assert write(kind=-1) == write(mode=8) == write(mode=_native.ROPE_TABLE) == write(rows=2) == invalid
     assert write(mode=_native.ROPE_ROWS, rows=5) == write(mode=_native.ROPE_ROWS | _native.ROPE_PREFILL) == invalid
     assert write(d=32) == write(packed=p + 1) == write(query=p + 2) == write(keys=p + 8) == unsupported
+
+
+@pytest.mark.parametrize("splits", [-1, 1025, (1 << 32) + 1])
+def test_interval_counts_refused(splits):
+    with pytest.raises(ValueError):
+        C._launch(0, 1, 8, 2, 64, 128, splits)

@@ -128,3 +128,9 @@ def test_entry_point_refuses_bad_handles():
     assert status(codes=1 << 12 | 8) == status(x=(1 << 12) + 1) == _native.FTK_ERR_UNSUPPORTED
     assert lib.ftk_w4_project_bf16(1 << 12, 128, None, 1e-6, None, None, 1 << 12, 1, None) == _native.FTK_ERR_INVALID
     assert lib.ftk_w4_dequantize_bf16(weight._handle, None, None) == _native.FTK_ERR_INVALID
+
+
+@pytest.mark.parametrize("shape,group", [((4, 64), 0), ((4, 64), -32), ((0, 64), 32), ((4, 0), 32)])
+def test_quantize_refusals(shape, group):
+    with pytest.raises(ValueError):
+        w4.quantize_w4(torch.ones(shape, dtype=torch.bfloat16), group)
