@@ -30,7 +30,7 @@ constexpr int kW4Chunk = 128;   // columns of a chunk
 constexpr int kW4Tile = 16;     // weight rows of a tile (SwiGLU: 8 gate rows and the 8 up rows beside them)
 constexpr int kW4MaxRows = 32;  // rows of x
 
-// A workgroup's waves: they split a row's chunks.
+// A workgroup's waves, which split a row's chunks (16 for a few short walks, see w4_shape).
 constexpr int kW4Waves = 8;
 
 // Builds of 128 registers, two workgroups to a CU: where x takes few of them, and one row with one scale to a chunk. (Three
@@ -41,7 +41,7 @@ constexpr bool w4_pairs(int held, int blocks, int subs, bool streamed, bool one)
 
 // The launch: `held` chunks per wave in registers (streamed: `held` at a time), `blocks` blocks of 16 operand rows.
 struct W4Shape {
-  int held, blocks, grid;
+  int held, blocks, grid, waves;
   bool streamed, one;  // passes; a single row of x
 };
 W4Shape w4_shape(W4Args& a, int subs, int cus);

@@ -15,7 +15,7 @@
 // row of the small ones the launch and the chain x, operand, first product, outputs -- 4096 x 1024 + norm 3.7 (2.2). From
 // about 8 rows on it is the vector unit: x becomes the operand in every workgroup (some 65 instructions for 8 elements
 // of a normalised row), and a tile's codes are unpacked once per row block (7 for 8 codes): 6144 x 4096 + norm at 16 rows
-// 10.7 (3.5), 24576 x 4096 + norm + SwiGLU at 8 / 16 / 24 rows 14.4 / 19.0 / 26.5 (9.6). An operand formed by a launch of
+// 10.0 (3.5), 24576 x 4096 + norm + SwiGLU at 8 / 16 / 24 rows 14.4 / 19.0 / 26.5 (9.6). An operand formed by a launch of
 // its own took that launch's 4 to 5 us again (16 rows of 6144 x 4096 13.3, 24 rows of 24576 x 4096 29.3).
 #include "ftk_w4_walk.h"
 
@@ -73,6 +73,12 @@ W4Shape w4_shape(W4Args& a, int subs, int cus) {
     const int all = cus * (w4_pairs(s.held, s.blocks, subs, s.streamed, s.one) ? 2 : 1) / a.row_blocks / 8 * 8;
     const int slots = all > 0 ? all : 8;
     rounds = (a.tiles + slots - 1) / slots;
+    // Four chunks to a wave and at most four tiles: 16 waves of two chunks each form x sooner and hide more. Longer walks
+    // pay for the 16 partial sums of each output (8 waves, 16: 6144 x 4096 + norm at 8 rows 8.4 us, 7.8, at 16 rows 9.5,
+    // 9.0; 4096 x 4096 at 8 rows 5.7, 5.0; 24576 x 4096 + norm at 8 rows 14.6, 15.3), and idle waves cost more than they
+    // hide (9497 x 2570 at 5 rows, 21 chunks, 6.9, 7.5).
+    s.waves = kW4Waves;
+    if (blocks == 1 && !s.one && need == 4 && rounds <= 4) s.waves = 16, s.held = 2;
     const int walkers = (a.tiles + rounds - 1) / rounds;
     s.grid = (walkers + 7) / 8 * 8 * a.row_blocks;
     return s;

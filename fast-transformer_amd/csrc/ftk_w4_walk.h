@@ -147,7 +147,7 @@ __device__ __forceinline__ float group_sum(float v) {
 
 }  // namespace w4
 
-// A workgroup walks tiles walker, walker + walkers, ... Its 8 waves split a tile's chunks (chunk = wave + 8 j), so
+// A workgroup walks tiles walker, walker + walkers, ... Its W waves split a tile's chunks (chunk = wave + W j), so
 // every wave needs its own chunks of x only. KC: chunks per wave in registers; CB: blocks of 16 operand rows. x is
 // the A operand and the weights the B operand: a lane's accumulators belong to one weight row, one scale serves them.
 // XS: more chunks than registers hold; a tile takes several passes, and x is read again for each.
@@ -160,11 +160,10 @@ __device__ __forceinline__ float group_sum(float v) {
 // One row with one scale to a chunk and at most 4 chunks takes 128 registers with PF = 1: two workgroups to a CU hide
 // more than two tiles in flight do (24576 x 4096 + norm 12.6 -> 12.1 us, 6144 x 4096 + norm 6.2 -> 6.0).
 // The weights of the next PF tiles are in flight; x goes out ahead of the first ones, since loads return in order.
-template <int KC, int CB, int S, bool ZP, bool XS, bool ONE>
-__global__ __launch_bounds__(64 * kW4Waves, (w4_pairs(KC, CB, S, XS, ONE) ? 4 : 2)) void w4_walk_kernel(W4Args a) {
+template <int KC, int CB, int S, bool ZP, bool XS, bool ONE, int W>
+__global__ __launch_bounds__(64 * W, (W == 16 || w4_pairs(KC, CB, S, XS, ONE) ? 4 : 2)) void w4_walk_kernel(W4Args a) {
   using namespace w4;
   static_assert(!ONE || CB == 1, "one row fills no block");
-  constexpr int W = kW4Waves;
   constexpr int PF = w4_pairs(KC, CB, S, XS, ONE) && KC > 2 ? 1 : (S == 4 ? KC * CB <= 4 : KC * CB <= 6) && !XS ? 2 : 1;
   constexpr int Q = ONE ? (KC + 3) / 4 : 1;  // pieces of the row per lane
   __shared__ float red[2][W][16 * CB][17];
@@ -508,20 +507,20 @@ __global__ __launch_bounds__(64 * kW4Waves, (w4_pairs(KC, CB, S, XS, ONE) ? 4 : 
 
 namespace w4 {
 
-template <int KC, int CB, int S, bool XS, bool ONE>
+template <int KC, int CB, int S, bool XS, bool ONE, int W = kW4Waves>
 void launch(const W4Args& a, const W4Shape& s, hipStream_t stream) {
   const int operands = (a.gain != nullptr ? 2 : 1) * a.rows;
-  const size_t lds = kW4Waves * 256 * (ONE ? (size_t)KC * operands : (size_t)16 * CB);
+  const size_t lds = W * 256 * (ONE ? (size_t)KC * operands : (size_t)16 * CB);
   if (a.zeros != nullptr)
-    hipLaunchKernelGGL((w4_walk_kernel<KC, CB, S, true, XS, ONE>), dim3(s.grid), dim3(64 * kW4Waves), lds, stream, a);
+    hipLaunchKernelGGL((w4_walk_kernel<KC, CB, S, true, XS, ONE, W>), dim3(s.grid), dim3(64 * W), lds, stream, a);
   else
-    hipLaunchKernelGGL((w4_walk_kernel<KC, CB, S, false, XS, ONE>), dim3(s.grid), dim3(64 * kW4Waves), lds, stream, a);
+    hipLaunchKernelGGL((w4_walk_kernel<KC, CB, S, false, XS, ONE, W>), dim3(s.grid), dim3(64 * W), lds, stream, a);
 }
 
 // Every launch that w4_shape makes.
 template <int S>
 hipError_t launch_shape(const W4Args& a, const W4Shape& s, hipStream_t stream) {
-  const int key = (s.one ? 2000 : 0) + (s.streamed ? 1000 : 0) + s.blocks * 100 + s.held;
+  const int key = (s.waves == 16 ? 4000 : 0) + (s.one ? 2000 : 0) + (s.streamed ? 1000 : 0) + s.blocks * 100 + s.held;
   if constexpr (S < 4) {
     if (key == 204) {
       launch<4, 2, S, false, false>(a, s, stream);
@@ -535,6 +534,7 @@ hipError_t launch_shape(const W4Args& a, const W4Shape& s, hipStream_t stream) {
     case 104: launch<4, 1, S, false, false>(a, s, stream); break;
     case 106: launch<(S < 4 ? 6 : 4), 1, S, false, false>(a, s, stream); break;
     case 108: launch<(S < 2 ? 8 : 4), 1, S, false, false>(a, s, stream); break;
+    case 4102: launch<2, 1, S, false, false, 16>(a, s, stream); break;
     case 1104: launch<4, 1, S, true, false>(a, s, stream); break;
     case 2101: launch<1, 1, S, false, true>(a, s, stream); break;
     case 2102: launch<2, 1, S, false, true>(a, s, stream); break;

@@ -113,6 +113,18 @@ LAUNCHES = [(1, 512, 1024), (7, 100, 2570), (16, 272, 4096), (32, 33, 512), (1, 
 @pytest.mark.parametrize("norm", [False, True])
 @pytest.mark.parametrize("m,n,k,group", [(17, 19001, 2200, 128), (24, 25003, 3130, 64), (32, 18800, 4096, 128)])
 def test_two_blocks_of_rows(m, n, k, group, norm, cuda):
+    check_rows(m, n, k, group, norm, cuda)
+
+
+# Short walks with four chunks to each of eight waves, which 16 waves take: whole and ragged rows, idle waves.
+@pytest.mark.parametrize("norm", [False, True])
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("m,n,k", [(2, 333, 3201), (7, 6150, 4096), (9, 40, 3977), (32, 1000, 3400)])
+def test_sixteen_waves(m, n, k, group, norm, cuda):
+    check_rows(m, n, k, group, norm, cuda)
+
+
+def check_rows(m, n, k, group, norm, cuda):
     weight, *parts = make(n, k, group, group == 64, cuda)
     x, r = inputs(m, k, cuda), inputs(m, n, cuda, 4)
     gain = (inputs(1, k, cuda, 3)[0].float() * 0.1 + 1).to(torch.bfloat16)
