@@ -32,17 +32,21 @@ constexpr int kW4MaxRows = 32;  // rows of x
 
 // A workgroup's waves, which split a row's chunks (16 for a few short walks, see w4_shape).
 constexpr int kW4Waves = 8;
+// Where x is: its chunks held in registers; or more than they hold, taken in passes, a tile's passes in turn or a batch's
+// tiles in turn for each pass.
+constexpr int kW4Held = 0, kW4Passes = 1, kW4Batches = 2;
+constexpr int kW4Turns = 8;  // tiles of a batch
 
 // Builds of 128 registers, two workgroups to a CU: where x takes few of them, and one row with one scale to a chunk. (Three
 // chunks held for several rows fit too, with one tile in flight instead of two: 9497 x 2570 at 5 rows 7.9 -> 8.3 us.)
-constexpr bool w4_pairs(int held, int blocks, int subs, bool streamed, bool one) {
-  return blocks == 1 && !streamed && (held <= 2 || (held <= 4 && subs == 1 && one));
+constexpr bool w4_pairs(int held, int blocks, int subs, int passes, bool one) {
+  return blocks == 1 && passes == kW4Held && (held <= 2 || (held <= 4 && subs == 1 && one));
 }
 
-// The launch: `held` chunks per wave in registers (streamed: `held` at a time), `blocks` blocks of 16 operand rows.
+// The launch: `held` chunks per wave in registers (of a pass: at a time), `blocks` blocks of 16 operand rows.
 struct W4Shape {
-  int held, blocks, grid, waves;
-  bool streamed, one;  // passes; a single row of x
+  int held, blocks, grid, waves, passes;  // passes: kW4Held, ...
+  bool one;                               // a single row of x
 };
 W4Shape w4_shape(W4Args& a, int subs, int cus);
 hipError_t launch_w4_s1(const W4Args& a, const W4Shape& s, hipStream_t stream);  // by groups per chunk

@@ -64,13 +64,13 @@ W4Shape w4_shape(W4Args& a, int subs, int cus) {
     a.row_blocks = (a.M + a.rows - 1) / a.rows;
     s.blocks = blocks;
     s.one = a.M == 1;
-    s.streamed = need > most_held;
+    s.passes = need > most_held ? kW4Passes : kW4Held;
     s.held = blocks == 2 ? 4 : s.one && subs < 4 ? 6 : 4;
-    if (blocks == 1 && !s.streamed)
+    if (blocks == 1 && s.passes == kW4Held)
       for (const int* h = held; (s.held = *h) < need; ++h) {}
     // One workgroup to a CU (two where its waves hold few chunks), as many for each row block, by eights; all walks as
     // even as they come.
-    const int all = cus * (w4_pairs(s.held, s.blocks, subs, s.streamed, s.one) ? 2 : 1) / a.row_blocks / 8 * 8;
+    const int all = cus * (w4_pairs(s.held, s.blocks, subs, s.passes, s.one) ? 2 : 1) / a.row_blocks / 8 * 8;
     const int slots = all > 0 ? all : 8;
     rounds = (a.tiles + slots - 1) / slots;
     // Four chunks to a wave and at most four tiles: 16 waves of two chunks each form x sooner and hide more. Longer walks
@@ -79,6 +79,10 @@ W4Shape w4_shape(W4Args& a, int subs, int cus) {
     // hide (9497 x 2570 at 5 rows, 21 chunks, 6.9, 7.5).
     s.waves = kW4Waves;
     if (blocks == 1 && !s.one && need == 4 && rounds <= 4) s.waves = 16, s.held = 2;
+    // Passes of several rows and more than one tile: the tiles of a batch take each pass in turn, so that a pass's x
+    // becomes the operand once a batch, not once a tile (a tile's passes in turn, batches: 16384 x 12288 at 32 rows 80 us,
+    // 41; 4096 x 12288 + norm at 16 rows 25.3, 19.0; a single tile, 4096 x 12288 at 16 rows, 13.6, 14.7).
+    if (s.passes == kW4Passes && !s.one && rounds > 1) s.passes = kW4Batches;
     const int walkers = (a.tiles + rounds - 1) / rounds;
     s.grid = (walkers + 7) / 8 * 8 * a.row_blocks;
     return s;

@@ -150,7 +150,8 @@ __device__ __forceinline__ float group_sum(float v) {
 // A workgroup walks tiles walker, walker + walkers, ... Its W waves split a tile's chunks (chunk = wave + W j), so
 // every wave needs its own chunks of x only. KC: chunks per wave in registers; CB: blocks of 16 operand rows. x is
 // the A operand and the weights the B operand: a lane's accumulators belong to one weight row, one scale serves them.
-// XS: more chunks than registers hold; a tile takes several passes, and x is read again for each.
+// XS: more chunks than registers hold. kW4Passes: a tile takes several passes, and x is read again for each. kW4Batches:
+// the tiles of a batch take a pass in turn, their sums so far in LDS, and x is read again for each batch and pass.
 // With a gain the operand rows are the rows' x gain as two BF16 addends (rows, then their low parts), and 1 / rms
 // joins in the epilogue: no product waits for the norm's sum, and x gain loses nothing.
 // Rows reach the operand through the wave's own part of LDS: read in the operand's layout, a load touches 16 rows x 64
@@ -160,13 +161,15 @@ __device__ __forceinline__ float group_sum(float v) {
 // One row with one scale to a chunk and at most 4 chunks takes 128 registers with PF = 1: two workgroups to a CU hide
 // more than two tiles in flight do (24576 x 4096 + norm 12.6 -> 12.1 us, 6144 x 4096 + norm 6.2 -> 6.0).
 // The weights of the next PF tiles are in flight; x goes out ahead of the first ones, since loads return in order.
-template <int KC, int CB, int S, bool ZP, bool XS, bool ONE, int W>
+template <int KC, int CB, int S, bool ZP, int XS, bool ONE, int W>
 __global__ __launch_bounds__(64 * W, (W == 16 || w4_pairs(KC, CB, S, XS, ONE) ? 4 : 2)) void w4_walk_kernel(W4Args a) {
   using namespace w4;
   static_assert(!ONE || CB == 1, "one row fills no block");
   constexpr int PF = w4_pairs(KC, CB, S, XS, ONE) && KC > 2 ? 1 : (S == 4 ? KC * CB <= 4 : KC * CB <= 6) && !XS ? 2 : 1;
   constexpr int Q = ONE ? (KC + 3) / 4 : 1;  // pieces of the row per lane
-  __shared__ float red[2][W][16 * CB][17];
+  constexpr bool TURNS = XS == kW4Batches, PASSES = XS == kW4Passes && !ONE;
+  constexpr int T = TURNS ? kW4Turns : 2;
+  __shared__ float red[T][W][16 * CB][17];
   __shared__ float ssq[W][16 * CB];
   __shared__ f32x4_t xsum[W][KC * S][4 * CB];  // per group: sums of the operand rows
   // ONE: pieces [W][KC 16][R]; else a chunk's [W][16 CB rows][16], piece p of row r at place p ^ (r % 16).
@@ -207,7 +210,7 @@ __global__ __launch_bounds__(64 * W, (W == 16 || w4_pairs(KC, CB, S, XS, ONE) ? 
     if constexpr (ZP) zp[f][j].load(t.zeros, (uint32_t)chunk * 16u + li);
   };
 
-  u32x4_t x[CB][XS && !ONE ? 1 : KC][4];
+  u32x4_t x[CB][PASSES ? 1 : KC][4];
   if constexpr (ONE) {
 #pragma unroll
     for (int j = 0; j < KC; ++j)
@@ -332,7 +335,7 @@ __global__ __launch_bounds__(64 * W, (W == 16 || w4_pairs(KC, CB, S, XS, ONE) ? 
       for (int b = 0; b < CB; ++b)
 #pragma unroll
         for (int s = 0; s < 4; ++s)
-          x[b][XS ? 0 : j][s] = chunk_lds[(16 * b + li) * 16 + ((4 * s + g) ^ li)];
+          x[b][PASSES ? 0 : j][s] = chunk_lds[(16 * b + li) * 16 + ((4 * s + g) ^ li)];
     }
   };
   auto keep_squares = [&]() {
@@ -356,21 +359,43 @@ __global__ __launch_bounds__(64 * W, (W == 16 || w4_pairs(KC, CB, S, XS, ONE) ? 
     for (int j = 0; j < KC; ++j) load_chunk(j, wave + W * j);
   }
   asm volatile("" ::: "memory");
-  // Steps (a tile's passes in turn, then the next tile's) PF ahead of the one computed: their tile and pass.
-  int load_tile = walker, load_pass = 0;
+  // Steps: a tile's passes in turn, then the next tile's. TURNS: a batch's tiles in turn, then their next pass, then the
+  // next batch. The loads are PF steps ahead of the one computed.
+  struct Step {
+    int tile, pass, first, at;  // at: the tile's place in the batch that begins with tile `first`
+  };
+  auto last_of_pass = [&](const Step& st) { return st.at + 1 == T || st.tile + walkers >= a.tiles; };
+  auto advance = [&](Step& st) {
+    if constexpr (TURNS) {
+      if (!last_of_pass(st)) {
+        st.tile += walkers;
+        ++st.at;
+        return;
+      }
+      if (++st.pass == passes) {
+        st.pass = 0;
+        st.first = st.tile + walkers;
+      }
+      st.tile = st.first;
+      st.at = 0;
+    } else if (!XS || ++st.pass == passes) {
+      st.pass = 0;
+      st.tile += walkers;
+      st.first = st.tile;
+    }
+  };
+  Step ahead = {walker, 0, walker, 0};
   Tile from = tile_of(walker);
   auto next_load = [&]() {
-    if (!XS || ++load_pass == passes) {
-      load_pass = 0;
-      load_tile += walkers;
-      from = tile_of(load_tile);
-    }
+    const int was = ahead.tile;
+    advance(ahead);
+    if (!XS || ahead.tile != was) from = tile_of(ahead.tile);
   };
 #pragma unroll
   for (int f = 0; f < PF; ++f) {
 #pragma unroll
     for (int j = 0; j < KC; ++j) {
-      load_weights(from, f, j, load_pass * KC * W + wave + W * j);
+      load_weights(from, f, j, ahead.pass * KC * W + wave + W * j);
       // (In the loop's order: a wait counts the loads behind the one it waits for, on this way into the loop as well.)
       __builtin_amdgcn_sched_barrier(0);
     }
@@ -379,25 +404,26 @@ __global__ __launch_bounds__(64 * W, (W == 16 || w4_pairs(KC, CB, S, XS, ONE) ? 
   if constexpr (!XS) {
     if constexpr (ONE) {
       form_pieces(0, true);
-      if (norm) keep_squares();
     } else {
 #pragma unroll
       for (int j = 0; j < KC; ++j) {
         form_chunk(j, wave + W * j, true);
         __builtin_amdgcn_sched_barrier(0);  // one chunk's temporaries at a time
       }
-      if (norm) keep_squares();
     }
+    if (norm) keep_squares();
   }
 
   __shared__ float inverse[16 * CB];  // 1 / rms of the rows, from the first tile on
-  int buf = 0, tile = walker, p = 0, turn = 0;
+  int buf = 0, turn = 0;
+  Step now = {walker, 0, walker, 0};
   f32x4_t acc[CB] = {};
-  while (tile < a.tiles) {
+  while (now.tile < a.tiles) {
 #pragma unroll
     for (int f = 0; f < PF; ++f) {
       // Past the walk's end a step computes nothing, but its loads (of nothing) go out: with an exit here the waits at
       // the loop's head would allow for the loads of this step only.
+      const int tile = now.tile, p = now.pass;
       const bool active = f == 0 || tile < a.tiles;
       // Many groups' sums stay in LDS: read for every tile (an index the compiler cannot see through), not kept in
       // registers over the walk.
@@ -409,9 +435,11 @@ __global__ __launch_bounds__(64 * W, (W == 16 || w4_pairs(KC, CB, S, XS, ONE) ? 
       }
 #pragma unroll
       for (int j = 0; j < KC; ++j) {
-        if constexpr (XS && !ONE) {
-          form_chunk(j, p * KC * W + wave + W * j, tile == walker);
-          load_chunk(j, (p + 1 == passes ? 0 : p + 1) * KC * W + wave + W * j);
+        if constexpr (TURNS || PASSES) {
+          if (PASSES || now.at == 0) {  // (the first of a batch's tiles brings the pass's x into the operand)
+            form_chunk(j, p * KC * W + wave + W * j, now.first == walker);
+            load_chunk(j, (p + 1 == passes ? 0 : p + 1) * KC * W + wave + W * j);
+          }
         }
         if (active) {
           float scale[S];
@@ -430,7 +458,7 @@ __global__ __launch_bounds__(64 * W, (W == 16 || w4_pairs(KC, CB, S, XS, ONE) ? 
               const uint32_t wv = w[f][j][i];
               const u32x4_t o = unpack(wv);
 #pragma unroll
-              for (int b = 0; b < CB; ++b) part[b] = mfma16x16x32(x[b][XS && !ONE ? 0 : j][i], o, part[b]);
+              for (int b = 0; b < CB; ++b) part[b] = mfma16x16x32(x[b][PASSES ? 0 : j][i], o, part[b]);
             }
 #pragma unroll
             for (int b = 0; b < CB; ++b) acc[b] += part[b] * scale[s];
@@ -440,21 +468,40 @@ __global__ __launch_bounds__(64 * W, (W == 16 || w4_pairs(KC, CB, S, XS, ONE) ? 
 #pragma unroll
           for (int s = 0; s < S; ++s) asm volatile("" ::"v"(scale[s]) : "memory");
         }
-        load_weights(from, f, j, load_pass * KC * W + wave + W * j);
+        load_weights(from, f, j, ahead.pass * KC * W + wave + W * j);
         __builtin_amdgcn_sched_barrier(0);
       }
       next_load();
       if constexpr (XS) {
-        if (active && ++p < passes) continue;
-        p = 0;
+        const Step done = now;
+        if (active) advance(now);
+        if constexpr (TURNS) {
+          // A tile's sums over the passes so far stay in its wave's place. (A batch's last tile may still be read for the
+          // outputs of the batch before; the others' readers have passed that tile's barrier.)
+          if (done.at + 1 == T && p == 0 && done.first != walker) lds_barrier();
+#pragma unroll
+          for (int b = 0; b < CB; ++b)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              float* const at = &red[done.at][wave][16 * b + 4 * g + r][li];
+              *at = p == 0 ? acc[b][r] : acc[b][r] + *at;
+              if (r == 3) acc[b] = f32x4_t{};
+            }
+          buf = done.at;
+        }
+        if (active && p + 1 < passes) continue;
+      } else {
+        if (active) advance(now);
       }
       if (!active) continue;
       // Element r of acc[b]: operand row 16 b + 4 g + r, weight row li of the tile.
+      if constexpr (!TURNS) {
 #pragma unroll
-      for (int b = 0; b < CB; ++b) {
+        for (int b = 0; b < CB; ++b) {
 #pragma unroll
-        for (int r = 0; r < 4; ++r) red[buf][wave][16 * b + 4 * g + r][li] = acc[b][r];
-        acc[b] = f32x4_t{};
+          for (int r = 0; r < 4; ++r) red[buf][wave][16 * b + 4 * g + r][li] = acc[b][r];
+          acc[b] = f32x4_t{};
+        }
       }
       if (XS && norm && tile == walker) keep_squares();
       lds_barrier();
@@ -500,14 +547,13 @@ __global__ __launch_bounds__(64 * W, (W == 16 || w4_pairs(KC, CB, S, XS, ONE) ? 
       }
       buf ^= 1;
       turn = (turn + 1) & (W - 1);
-      tile += walkers;
     }
   }
 }
 
 namespace w4 {
 
-template <int KC, int CB, int S, bool XS, bool ONE, int W = kW4Waves>
+template <int KC, int CB, int S, int XS, bool ONE, int W = kW4Waves>
 void launch(const W4Args& a, const W4Shape& s, hipStream_t stream) {
   const int operands = (a.gain != nullptr ? 2 : 1) * a.rows;
   const size_t lds = W * 256 * (ONE ? (size_t)KC * operands : (size_t)16 * CB);
@@ -520,30 +566,31 @@ void launch(const W4Args& a, const W4Shape& s, hipStream_t stream) {
 // Every launch that w4_shape makes.
 template <int S>
 hipError_t launch_shape(const W4Args& a, const W4Shape& s, hipStream_t stream) {
-  const int key = (s.waves == 16 ? 4000 : 0) + (s.one ? 2000 : 0) + (s.streamed ? 1000 : 0) + s.blocks * 100 + s.held;
+  const int key = (s.waves == 16 ? 8000 : 0) + (s.one ? 4000 : 0) + 1000 * s.passes + s.blocks * 100 + s.held;
   if constexpr (S < 4) {
     if (key == 204) {
-      launch<4, 2, S, false, false>(a, s, stream);
+      launch<4, 2, S, kW4Held, false>(a, s, stream);
       return hipGetLastError();
     }
   }
   switch (key) {
-    case 101: launch<1, 1, S, false, false>(a, s, stream); break;
-    case 102: launch<2, 1, S, false, false>(a, s, stream); break;
-    case 103: launch<3, 1, S, false, false>(a, s, stream); break;
-    case 104: launch<4, 1, S, false, false>(a, s, stream); break;
-    case 106: launch<(S < 4 ? 6 : 4), 1, S, false, false>(a, s, stream); break;
-    case 108: launch<(S < 2 ? 8 : 4), 1, S, false, false>(a, s, stream); break;
-    case 4102: launch<2, 1, S, false, false, 16>(a, s, stream); break;
-    case 1104: launch<4, 1, S, true, false>(a, s, stream); break;
-    case 2101: launch<1, 1, S, false, true>(a, s, stream); break;
-    case 2102: launch<2, 1, S, false, true>(a, s, stream); break;
-    case 2103: launch<3, 1, S, false, true>(a, s, stream); break;
-    case 2104: launch<4, 1, S, false, true>(a, s, stream); break;
-    case 2106: launch<(S < 4 ? 6 : 4), 1, S, false, true>(a, s, stream); break;
-    case 2108: launch<(S < 2 ? 8 : 4), 1, S, false, true>(a, s, stream); break;
-    case 3106: launch<(S < 4 ? 6 : 4), 1, S, true, true>(a, s, stream); break;
-    case 3104: launch<4, 1, S, true, true>(a, s, stream); break;
+    case 101: launch<1, 1, S, kW4Held, false>(a, s, stream); break;
+    case 102: launch<2, 1, S, kW4Held, false>(a, s, stream); break;
+    case 103: launch<3, 1, S, kW4Held, false>(a, s, stream); break;
+    case 104: launch<4, 1, S, kW4Held, false>(a, s, stream); break;
+    case 106: launch<(S < 4 ? 6 : 4), 1, S, kW4Held, false>(a, s, stream); break;
+    case 108: launch<(S < 2 ? 8 : 4), 1, S, kW4Held, false>(a, s, stream); break;
+    case 8102: launch<2, 1, S, kW4Held, false, 16>(a, s, stream); break;
+    case 1104: launch<4, 1, S, kW4Passes, false>(a, s, stream); break;
+    case 2104: launch<(S < 4 ? 4 : 3), 1, S, kW4Batches, false>(a, s, stream); break;
+    case 4101: launch<1, 1, S, kW4Held, true>(a, s, stream); break;
+    case 4102: launch<2, 1, S, kW4Held, true>(a, s, stream); break;
+    case 4103: launch<3, 1, S, kW4Held, true>(a, s, stream); break;
+    case 4104: launch<4, 1, S, kW4Held, true>(a, s, stream); break;
+    case 4106: launch<(S < 4 ? 6 : 4), 1, S, kW4Held, true>(a, s, stream); break;
+    case 4108: launch<(S < 2 ? 8 : 4), 1, S, kW4Held, true>(a, s, stream); break;
+    case 5106: launch<(S < 4 ? 6 : 4), 1, S, kW4Passes, true>(a, s, stream); break;
+    case 5104: launch<4, 1, S, kW4Passes, true>(a, s, stream); break;
     default: return hipErrorInvalidValue;
   }
   return hipGetLastError();

@@ -124,6 +124,15 @@ def test_sixteen_waves(m, n, k, group, norm, cuda):
     check_rows(m, n, k, group, norm, cuda)
 
 
+# Rows of several passes whose walks take two tiles, a batch and one more, two batches and more (32 rows under a norm and
+# without: a workgroup walks n / 1024 and n / 2048 tiles).
+@pytest.mark.parametrize("norm", [False, True])
+@pytest.mark.parametrize("m,n,k,group", [(32, 1500, 8300, 128), (32, 8700, 6200, 64), (32, 17003, 4300, 32),
+                                         (9, 4200, 12288, 128)])
+def test_batches_of_passes(m, n, k, group, norm, cuda):
+    check_rows(m, n, k, group, norm, cuda)
+
+
 def check_rows(m, n, k, group, norm, cuda):
     weight, *parts = make(n, k, group, group == 64, cuda)
     x, r = inputs(m, k, cuda), inputs(m, n, cuda, 4)
