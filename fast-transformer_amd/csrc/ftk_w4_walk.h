@@ -582,6 +582,7 @@ hipError_t launch_shape(const W4Args& a, const W4Shape& s, hipStream_t stream) {
     case 108: launch<(S < 2 ? 8 : 4), 1, S, kW4Held, false>(a, s, stream); break;
     case 8102: launch<2, 1, S, kW4Held, false, 16>(a, s, stream); break;
     case 1104: launch<4, 1, S, kW4Passes, false>(a, s, stream); break;
+    // (Four groups to a chunk: three chunks of a pass, four would spill.)
     case 2104: launch<(S < 4 ? 4 : 3), 1, S, kW4Batches, false>(a, s, stream); break;
     case 4101: launch<1, 1, S, kW4Held, true>(a, s, stream); break;
     case 4102: launch<2, 1, S, kW4Held, true>(a, s, stream); break;
@@ -589,8 +590,8 @@ hipError_t launch_shape(const W4Args& a, const W4Shape& s, hipStream_t stream) {
     case 4104: launch<4, 1, S, kW4Held, true>(a, s, stream); break;
     case 4106: launch<(S < 4 ? 6 : 4), 1, S, kW4Held, true>(a, s, stream); break;
     case 4108: launch<(S < 2 ? 8 : 4), 1, S, kW4Held, true>(a, s, stream); break;
+    case 5104:
     case 5106: launch<(S < 4 ? 6 : 4), 1, S, kW4Passes, true>(a, s, stream); break;
-    case 5104: launch<4, 1, S, kW4Passes, true>(a, s, stream); break;
     default: return hipErrorInvalidValue;
   }
   return hipGetLastError();
